@@ -1,0 +1,828 @@
+// Causal attention of ragged query runs over a block cache of e4m3 codes with one scale per block and head (fa_cache.h: layout).
+//
+//   request b: n = cu_q[b+1] - cu_q[b] query tokens, the last n of its len = seq_lens[b] tokens; token i sees the keys below limit = len - n + i + 1.
+//   S = scale (q . code_k) scale_k,  O = sum_k exp(S - max) scale_v code_v / sum_k exp(S - max);  a row that sees no key gives zeros.
+//
+// Query rows of one key/value head are packed (token, head of its group), token first, so that a grouped head's codes are read and
+// converted once for all its query heads.  The unit of work is 64 tokens.  Products run transposed on v_mfma_f32_16x16x32, S^T = K Q^T and
+// O^T = V^T P^T: a query row is a lane's column, so that its maximum, sum and rescale are per-lane values, and the layouts are chosen so that nothing
+// moves between lanes on the way:
+//   * row `r` of key tile t (16 keys) is key 16 (r >> 2) + 4 t + (r & 3) of the unit: a lane's four results of the four tiles are the sixteen
+//     CONSECUTIVE keys 16 (lane >> 4) .. + 15, which is what the B operand of the second product wants of that lane (two products of 32 keys);
+//   * the value cache is token-inner, so the matching A operand (column d, those sixteen keys) is one 16-byte load, as is a key row's share.
+// e4m3 -> 16-bit is exact, one instruction per two values.  A unit's products of codes start from zero and are added as O += scale_v acc: the
+// scale multiplies in 32 bits, and P <= 1 is rounded once to the operand type as in the kernels for 16-bit operands.  Blocks shorter than a
+// unit bring several value scales into one product: P is then multiplied by scale_v / (largest scale_v of the unit) before it is rounded.
+// Maximum, sum and O are 32-bit.
+//
+// Two kernels:
+//   row kernel   few rows per key/value head (a decoding step): bound by the cache's bytes.  Codes go from memory straight into
+//                registers; a wave takes every fourth unit, the next unit's loads are in flight under the current one's arithmetic.  The
+//                grid is fixed; the units of all (request, head, row tile) are one line that is cut into equal ranges on the device, from the
+//                lengths there: no length is known to the host, and one long request fills the chip.  A (request, head, row tile) inside one range
+//                is finished there; one that crosses ranges leaves unnormalised partial sums that the join kernel adds in order.
+//   tile kernel  128 rows per workgroup, 64 above head dim 128 (prompts): bound by the matrix pipe.  Four waves share a unit's operands,
+//                converted once into LDS in the very order in which the lanes read them.  Grids too small for the chip cut every tile's
+//                key range into `splits` parts.
+// Stale codes behind a request's end are cleared before they meet a zero weight (0 * NaN), and a NaN code that only some rows of a unit may
+// see reaches those rows alone.
+#include <hip/hip_runtime.h>
+
+#include "fa_cache.h"
+#include "fa_device.h"
+
+namespace fa {
+namespace {
+
+typedef unsigned u32x2c __attribute__((ext_vector_type(2)));
+
+template <typename T> struct Code;
+template <> struct Code<__bf16> {
+    static __device__ __forceinline__ unsigned lo(unsigned w) { return __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, false)); }
+    static __device__ __forceinline__ unsigned hi(unsigned w) { return __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, true)); }
+};
+template <> struct Code<_Float16> {
+    static __device__ __forceinline__ unsigned lo(unsigned w) { return __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.0f, false)); }
+    static __device__ __forceinline__ unsigned hi(unsigned w) { return __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.0f, true)); }
+};
+// eight codes -> one operand fragment
+template <typename T>
+__device__ __forceinline__ typename Elt<T>::vec8 fragment(unsigned a, unsigned b) {
+    const u32x4 v = {Code<T>::lo(a), Code<T>::hi(a), Code<T>::lo(b), Code<T>::hi(b)};
+    return __builtin_bit_cast(typename Elt<T>::vec8, v);
+}
+template <typename T>
+__device__ __forceinline__ unsigned pack2(float a, float b) {
+    typedef T vec2 __attribute__((ext_vector_type(2)));
+    const vec2 v = {(T)a, (T)b};
+    return __builtin_bit_cast(unsigned, v);
+}
+// the four 16-lane groups of a wave hold parts of the same 16 rows: maximum / sum over the groups, in every lane
+__device__ __forceinline__ HalfPair group_exchange(float x) {
+    const unsigned u = __builtin_bit_cast(unsigned, x);
+    const auto r = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+    const unsigned r0 = r[0], r1 = r[1];
+    return {__builtin_bit_cast(float, r0), __builtin_bit_cast(float, r1)};
+}
+__device__ __forceinline__ float rows_max(float x) {
+    const HalfPair p = group_exchange(x);
+    x = __builtin_fmaxf(p.lo, p.hi);
+    const HalfPair h = half_exchange(x);
+    return __builtin_fmaxf(h.lo, h.hi);
+}
+__device__ __forceinline__ float rows_sum(float x) {
+    const HalfPair p = group_exchange(x);
+    x = p.lo + p.hi;
+    const HalfPair h = half_exchange(x);
+    return h.lo + h.hi;
+}
+// codes of the keys at and behind `valid` (of the sixteen in v) cleared
+__device__ __forceinline__ u32x4 clear_behind(u32x4 v, int valid) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int n = valid - 4 * i;
+        v[i] = n >= 4 ? v[i] : n <= 0 ? 0u : v[i] & (0xffffffffu >> (8 * (4 - n)));
+    }
+    return v;
+}
+
+__device__ __forceinline__ bool has_nan(u32x4 v) {
+    unsigned any = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) any |= ((v[i] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
+    return any != 0;
+}
+// the NaN codes of v cleared; which of the sixteen they were
+__device__ __forceinline__ unsigned take_nan(u32x4& v) {
+    unsigned bits = 0;
+    asm volatile("" : "+v"(v));                // (else has_nan's terms are kept for all of a lane's codes)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const unsigned n = (((v[i] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) >> 7;     // 1 in every NaN byte
+        v[i] &= ~(n * 0xffu);
+        bits |= ((n | n >> 7 | n >> 14 | n >> 21) & 0xfu) << (4 * i);
+    }
+    return bits;
+}
+
+// ---- a request as every kernel here sees it: all indexes held inside what the caller's tensors have ----------------------------------------
+struct Request {
+    int first, n, len, units;
+};
+__device__ __forceinline__ Request request_of(const CacheAttnParams& p, int b) {
+    Request r;
+    const int a = min(max(p.cu_q[b], 0), p.T), e = min(max(p.cu_q[b + 1], a), p.T);
+    const long long room = (long long)p.width << p.shift;
+    r.first = a;
+    r.n = e - a;
+    r.len = max(p.seq_lens[b], 0);
+    r.len = r.len < room ? r.len : (int)room;
+    r.units = max(1, (int)(((long long)r.len + 63) >> 6));
+    return r;
+}
+
+// Every workgroup finds its place by itself: `items(b)` summed over the requests (each thread a stretch of them), `want(total)` names the item to
+// find, and the stretch that holds it is walked.  prefix (or null) receives the sums.
+__device__ __forceinline__ long long uniform(long long x) {
+    const unsigned lo = (unsigned)__builtin_amdgcn_readfirstlane((int)x), hi = (unsigned)__builtin_amdgcn_readfirstlane((int)(x >> 32));
+    return (long long)((unsigned long long)hi << 32 | lo);
+}
+struct Place {
+    int b;
+    long long off, total;
+};
+template <int NT, typename Items, typename Want>
+__device__ __forceinline__ Place find_place(int B, Items items, Want want, long long* prefix) {
+    __shared__ long long sums[NT / 64 + 1];
+    __shared__ Place found;
+    const int tid = (int)threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int per = (B + NT - 1) / NT, from = min(tid * per, B), to = min(from + per, B);
+    long long mine = 0;
+    for (int b = from; b < to; ++b) mine += items(b);
+    long long incl = mine;
+    for (int d = 1; d < 64; d *= 2) {
+        const long long y = __shfl_up(incl, d);
+        if (lane >= d) incl += y;
+    }
+    if (lane == 63) sums[wave] = incl;
+    __syncthreads();
+    long long before = incl - mine, total = 0;
+    for (int w = 0; w < NT / 64; ++w) {
+        if (w < wave) before += sums[w];
+        total += sums[w];
+    }
+    total = uniform(total);
+    const long long x = want(total);
+    if (x >= before && x < before + mine) {
+        long long at = before;
+        int b = from;
+        for (;; ++b) {
+            const long long n = items(b);
+            if (x < at + n) break;
+            at += n;
+        }
+        found.b = b;
+        found.off = x - at;
+    }
+    if (prefix) {
+        long long at = before;
+        for (int b = from; b < to; ++b) { prefix[b] = at; at += items(b); }
+        if (tid == 0) prefix[B] = total;
+    }
+    __syncthreads();
+    Place f;
+    f.b = __builtin_amdgcn_readfirstlane(found.b);
+    f.off = uniform(found.off);
+    f.total = total;
+    return f;
+}
+
+// a value that the compiler may not form ahead of its use: what is derived from it is not kept in registers round a loop
+__device__ __forceinline__ int fresh_scalar(int x) { asm volatile("" : "+s"(x)); return x; }
+__device__ __forceinline__ int fresh_lane(int x) { asm volatile("" : "+v"(x)); return x; }
+
+// ---- the arithmetic of one unit for the 16 NR rows of a wave --------------------------------------------------------------------------------
+template <typename T, int W, int NR>
+struct RowState {
+    static constexpr int NC = W / 32, ND = W / 16;       // k-steps of Q K^T; 16-column tiles of O
+    using vec8 = typename Elt<T>::vec8;
+    vec8 q[NR][NC];
+    float o[NR][ND][4];                                  // (scalars: as vectors, every conditional change copies them)
+    float m[NR], l[NR];
+    int limit[NR];                                       // keys that the lane's row sees
+    int limit_min, limit_max;                            // over the wave's rows (uniform)
+    unsigned long long nan[NR];                          // bit 4 d + i: o[r][d][i] saw a NaN value (note_nan)
+
+    __device__ __forceinline__ void clear() {
+#pragma unroll
+        for (int r = 0; r < NR; ++r) {
+            m[r] = -INFINITY;
+            l[r] = 0.f;
+            nan[r] = 0;
+#pragma unroll
+            for (int d = 0; d < ND; ++d)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) o[r][d][i] = 0.f;
+        }
+    }
+    // rows row0 .. row0 + 16 NR - 1 of (request, key/value head h)
+    __device__ __forceinline__ void load(const CacheAttnParams& p, const Request& rq, int h, int row0, int lane) {
+        const int col = lane & 15, lg = lane >> 4, rows = rq.n * p.group;
+        const int i0 = row0 / p.group, i1 = min(row0 + 16 * NR, rows) - 1;
+        limit_min = rq.len - rq.n + i0 + 1;
+        limit_max = i1 >= row0 ? rq.len - rq.n + i1 / p.group + 1 : limit_min;
+#pragma unroll
+        for (int r = 0; r < NR; ++r) {
+            const int row = row0 + 16 * r + col;
+            const bool in = row < rows;
+            const int i = in ? row / p.group : 0, g = in ? row - i * p.group : 0;
+            limit[r] = in ? rq.len - rq.n + i + 1 : limit_min;
+            const T* src = (const T*)p.q + (int64_t)(rq.first + i) * p.q_st + (int64_t)(h * p.group + g) * p.q_sh;
+#pragma unroll
+            for (int c = 0; c < NC; ++c) {
+                const int d = 64 * (c >> 1) + 16 * lg + 8 * (c & 1);
+                u32x4 v = {0, 0, 0, 0};
+                if (in && d < p.D) v = *(const u32x4*)(src + d);
+                q[r][c] = __builtin_bit_cast(vec8, v);
+            }
+        }
+    }
+    // key(t, c): fragment c of key tile t; value(d, u): fragment of columns 16 d .., keys 8 u .. + 7 of every lane's sixteen.  kf: scale_k times the softmax
+    // scale in powers of two, and dead: whether the lane's sixteen keys are masked altogether; vs: the unit's value scale, ratio: the lane's share of it
+    template <typename Key>
+    __device__ __forceinline__ void scores(Key key, f32x4 (&s)[NR][4]) const {
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+#pragma unroll
+            for (int r = 0; r < NR; ++r) s[r][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int c = 0; c < NC; ++c) {
+                const vec8 a = key(t, c);
+#pragma unroll
+                for (int r = 0; r < NR; ++r) s[r][t] = Elt<T>::mfma16(a, q[r][c], s[r][t]);
+            }
+            __builtin_amdgcn_sched_barrier(0);           // (else every tile's conversions are hoisted and the registers spill)
+        }
+    }
+    template <bool SMALL>
+    __device__ __forceinline__ void softmax(f32x4 (&s)[NR][4], vec8 (&w)[NR][2], int key0, float kf, bool dead, float ratio, bool boundary) {
+#pragma unroll
+        for (int r = 0; r < NR; ++r) {
+            float top = -INFINITY;
+#pragma unroll
+            for (int t = 0; t < 4; ++t) s[r][t] *= kf;
+            if (boundary || SMALL) {
+                const int see = dead ? 0 : limit[r] - key0;        // the lane's keys are key0 .. key0 + 15
+#pragma unroll
+                for (int t = 0; t < 4; ++t)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) s[r][t][i] = 4 * t + i < see ? s[r][t][i] : -INFINITY;
+            }
+#pragma unroll
+            for (int t = 0; t < 4; ++t)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) top = __builtin_fmaxf(top, s[r][t][i]);
+            top = rows_max(top);
+            const float now = __builtin_fmaxf(m[r], top), base = now == -INFINITY ? 0.f : now;
+            if (__any(now > m[r])) {
+                const float alpha = fast_exp2(m[r] - base);
+                l[r] *= alpha;
+#pragma unroll
+                for (int d = 0; d < ND; ++d)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) o[r][d][i] *= alpha;
+                m[r] = now;
+            }
+            float sum = 0.f;
+            unsigned u[8];
+#pragma unroll
+            for (int t = 0; t < 4; ++t) {
+                float e[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    e[i] = fast_exp2(s[r][t][i] - base);
+                    sum += e[i];
+                    if constexpr (SMALL) e[i] *= ratio;
+                }
+                u[2 * t] = pack2<T>(e[0], e[1]);
+                u[2 * t + 1] = pack2<T>(e[2], e[3]);
+            }
+            l[r] += sum;
+            const u32x4 a = {u[0], u[1], u[2], u[3]}, b = {u[4], u[5], u[6], u[7]};
+            w[r][0] = __builtin_bit_cast(vec8, a);
+            w[r][1] = __builtin_bit_cast(vec8, b);
+        }
+    }
+    template <int D0, int D1, typename Value>
+    __device__ __forceinline__ void values(Value value, const vec8 (&w)[NR][2], float vs) {
+        const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int d = D0; d < D1; ++d) {
+            const vec8 a = value(d, 0), b = value(d, 1);
+#pragma unroll
+            for (int r = 0; r < NR; ++r) {
+                f32x4 acc = Elt<T>::mfma16(a, w[r][0], zero);
+                acc = Elt<T>::mfma16(b, w[r][1], acc);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) o[r][d][i] = __builtin_fmaf(acc[i], vs, o[r][d][i]);
+                // (pinned here: the compiler moves these sums behind the loop's last branch and keeps every product's registers until then)
+                asm volatile("" : "+v"(o[r][d][0]), "+v"(o[r][d][1]), "+v"(o[r][d][2]), "+v"(o[r][d][3]));
+            }
+            if (NR * W > 128 || d % 2) __builtin_amdgcn_sched_barrier(0);
+        }
+    }
+    // A unit that some rows see only in part holds NaN values: they were taken out of the operands (take_nan) and are noted for the rows that see
+    // them; keys[column]: the unit's keys with NaN in that column
+    __device__ __forceinline__ void note_nan(const unsigned long long* keys, int unit, int lg) {
+        keys += 4 * fresh_lane(lg);
+#pragma unroll 1
+        for (int e = 0; e < 4 * ND; ++e) {
+            const unsigned long long k = keys[16 * (e >> 2) + (e & 3)];
+#pragma unroll
+            for (int r = 0; r < NR; ++r) {
+                const int see = limit[r] - 64 * unit;
+                const unsigned long long seen = see <= 0 ? 0ull : see >= 64 ? ~0ull : (1ull << see) - 1;
+                nan[r] |= (unsigned long long)((k & seen) != 0) << e;
+            }
+        }
+    }
+    __device__ __forceinline__ void put_nan() {
+#pragma unroll
+        for (int r = 0; r < NR; ++r) {
+            if (!__any(nan[r] != 0)) continue;
+#pragma unroll
+            for (int d = 0; d < ND; ++d)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) o[r][d][i] = (nan[r] >> (4 * d + i)) & 1 ? __builtin_nanf("") : o[r][d][i];
+        }
+    }
+    // O / l of rows row0 .. into the output
+    __device__ __forceinline__ void store(const CacheAttnParams& p, const Request& rq, int h, int row0, int lane, const float (&sum)[NR]) const {
+        const int col = lane & 15, lg = lane >> 4, rows = rq.n * p.group;
+#pragma unroll
+        for (int r = 0; r < NR; ++r) {
+            const int row = row0 + 16 * r + col;
+            if (row >= rows) continue;
+            const int i = row / p.group, g = row - i * p.group;
+            T* dst = (T*)p.o + (int64_t)(rq.first + i) * p.o_st + (int64_t)(h * p.group + g) * p.o_sh;
+            const float inv = sum[r] == 0.f ? 0.f : 1.0f / sum[r];
+#pragma unroll
+            for (int d = 0; d < ND; ++d) {
+                const int at = 16 * d + 4 * lg;
+                if (at >= p.D) continue;
+                const float* v = o[r][d];
+                *(u32x2c*)(dst + at) = u32x2c{pack2<T>(v[0] * inv, v[1] * inv), pack2<T>(v[2] * inv, v[3] * inv)};
+            }
+        }
+    }
+    // unnormalised sums into a workspace slot of `rows16` rows, from its row `at` on
+    __device__ __forceinline__ void park(const CacheAttnParams& p, long long slot, int rows16, int at, int lane, const float (&sum)[NR], const float (&top)[NR]) const {
+        const int col = lane & 15, lg = lane >> 4;
+#pragma unroll
+        for (int r = 0; r < NR; ++r) {
+            const long long row = slot * rows16 + at + 16 * r + col;
+            if (lg == 0) { p.ws_ml[2 * row] = top[r]; p.ws_ml[2 * row + 1] = sum[r]; }
+#pragma unroll
+            for (int d = 0; d < ND; ++d) *(f32x4*)(p.ws_o + row * W + 16 * d + 4 * lg) = f32x4{o[r][d][0], o[r][d][1], o[r][d][2], o[r][d][3]};
+        }
+    }
+};
+
+// the block of a token index, -1 where the table has none that exists
+__device__ __forceinline__ int block_at(const CacheAttnParams& p, const int* table, int index) {
+    const int id = index < p.width ? table[index] : -1;
+    return (unsigned)id < (unsigned)p.num_blocks ? id : -1;
+}
+
+// Where a lane finds its codes of a unit, the scales, and whether its keys exist.  Blocks of a unit and more: base addresses are uniform and the
+// lane's part is a 32-bit offset that all units share; smaller blocks: the lane's own addresses.
+template <bool SMALL>
+struct UnitAt {
+    const uint8_t* k;
+    const uint8_t* v;
+    float kf, vs, ratio;
+    bool dead, none;          // the lane's sixteen keys have no block; the unit has none at all (uniform)
+    __device__ __forceinline__ void find(const CacheAttnParams& p, const int* table, int len, int u, int h, int W, int lane) {
+        const int lg = lane >> 4, wk = lane & 15, P = 1 << p.shift, first = 64 * u;
+        if constexpr (!SMALL) {
+            const int id = first < len ? block_at(p, table, first >> p.shift) : -1;
+            none = id < 0;
+            dead = none;
+            const long long blk = none ? 0 : id;
+            const int in = first & (P - 1);
+            k = p.k + blk * p.k_bs + (int64_t)(h * P + in) * W;
+            v = p.v + blk * p.v_bs + (int64_t)h * P * W + in;
+            kf = none ? 0.f : p.ks[blk * p.ks_bs + h] * p.scale_log2;
+            vs = none ? 0.f : p.vs[blk * p.vs_bs + h];
+            ratio = 1.f;
+        } else {
+            const int kk = first + 16 * (wk >> 2), vk = first + 16 * lg;
+            const int kid = kk < len ? block_at(p, table, kk >> p.shift) : -1;
+            const int vid = vk < len ? block_at(p, table, vk >> p.shift) : -1;
+            dead = vid < 0;
+            none = !__any(!dead);
+            const long long kb = kid < 0 ? 0 : kid, vb = vid < 0 ? 0 : vid;
+            k = p.k + kb * p.k_bs + (int64_t)(h * P + (kk & (P - 1))) * W;
+            v = p.v + vb * p.v_bs + (int64_t)h * P * W + (vk & (P - 1));
+            kf = dead ? 0.f : p.ks[vb * p.ks_bs + h] * p.scale_log2;
+            const float mine = dead ? 0.f : p.vs[vb * p.vs_bs + h];
+            vs = rows_max(mine);
+            ratio = vs > 0.f ? mine / vs : 0.f;
+        }
+    }
+    // byte offset of key tile 0's row of this lane, and of its row of value column 0
+    static __device__ __forceinline__ unsigned key_lane(int W, int lane) {
+        const int wk = lane & 15, lg = lane >> 4;
+        return (unsigned)(((SMALL ? 0 : 16 * (wk >> 2)) + (wk & 3)) * W + 16 * lg);
+    }
+    static __device__ __forceinline__ unsigned value_lane(int shift, int lane) {
+        return (unsigned)(((lane & 15) << shift) + (SMALL ? 0 : 16 * (lane >> 4)));
+    }
+};
+
+// ---- row kernel ---------------------------------------------------------------------------------------------------------------------------
+__device__ __forceinline__ long long row_items(const CacheAttnParams& p, const Request& rq, int rows16) {
+    const int tiles = (rq.n * p.group + rows16 - 1) / rows16;
+    return (long long)tiles * p.Hkv * rq.units;
+}
+__device__ __forceinline__ long long range_of(const CacheAttnParams& p, long long total) {
+    const long long per = (total + p.grid - 1) / p.grid;
+    return per > p.min_units ? per : p.min_units;
+}
+
+template <typename T, int W, int NR, bool SMALL>
+__global__ __launch_bounds__(256, 2) void cache_rows_kernel(CacheAttnParams p) {
+    using State = RowState<T, W, NR>;
+    constexpr int ND = State::ND, NK = W / 64, ROWS = 16 * NR;
+    // the next unit's codes are fetched under this one's arithmetic where the registers hold them beside O; else a unit's value columns are
+    // taken in parts
+    constexpr bool AHEAD = W * NR <= 128;
+    constexpr int VN = AHEAD ? ND : W > 192 && SMALL ? ND / 8 : W * NR > 192 ? ND / 4 : ND / 2;
+    __shared__ __align__(8) unsigned short nan_keys[4][4 * W];     // [wave][column][16-key group]
+    __shared__ f32x4 join_o[2][NR * ND * 64];
+    __shared__ float join_m[4][ROWS], join_l[4][ROWS];
+    const int lane = (int)threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+    const int lg = lane >> 4, wk = lane & 15;
+    long long range = 1, start = 0;
+    const Place at = find_place<256>(p.B, [&](int b) { return row_items(p, request_of(p, b), ROWS); },
+                                     [&](long long total) { range = range_of(p, total); start = range * (long long)blockIdx.x; return start; },
+                                     blockIdx.x == 0 ? p.ws_prefix : nullptr);
+    if (start >= at.total) return;
+    const long long end = start + range < at.total ? start + range : at.total;
+    int b = at.b;
+    long long off = at.off, cur = start;
+    const unsigned key_off = UnitAt<SMALL>::key_lane(W, lane), value_off = UnitAt<SMALL>::value_lane(p.shift, lane);
+    State st;
+    while (cur < end) {
+        const Request rq = request_of(p, b);
+        const int tiles = (rq.n * p.group + ROWS - 1) / ROWS;
+        const long long items = (long long)tiles * p.Hkv * rq.units;
+        if (off >= items) { ++b; off = 0; continue; }      // (the next request with rows; there is one, cur < end)
+        const int ht = (int)(off / rq.units), u0 = (int)(off - (long long)ht * rq.units);
+        const int h = ht / tiles, row0 = (ht - h * tiles) * ROWS;
+        const int u1 = (int)(u0 + (end - cur) < rq.units ? u0 + (end - cur) : rq.units);
+        const bool whole = u0 == 0 && u1 == rq.units;
+        const int* table = p.tables + (int64_t)b * p.table_stride;
+        st.load(p, rq, h, row0, lane);
+        st.clear();
+        u32x4 kr[4][NK], vr[VN];
+        UnitAt<SMALL> here, next;
+        const auto load_keys = [&](const UnitAt<SMALL>& a) {
+#pragma unroll
+            for (int t = 0; t < 4; ++t)
+#pragma unroll
+                for (int i = 0; i < NK; ++i) kr[t][i] = *(const u32x4*)(a.k + (4 * t * W + 64 * i) + key_off);
+        };
+        const auto drop_keys = [&]() {                     // (else the last unit's keys stay in registers for a round that never comes)
+#pragma unroll
+            for (int t = 0; t < 4; ++t)
+#pragma unroll
+                for (int i = 0; i < NK; ++i) kr[t][i] = __builtin_nondeterministic_value(kr[t][i]);
+        };
+        const auto load_values = [&](const UnitAt<SMALL>& a, int d0) {
+            const int step = fresh_scalar(16 << p.shift);
+#pragma unroll
+            for (int d = 0; d < VN; ++d) vr[d] = *(const u32x4*)(a.v + (d0 + d) * step + value_off);
+        };
+        int u = u0 + wave;
+        if (u < u1) {
+            here.find(p, table, rq.len, u, h, W, lane);
+            load_keys(here);
+            if (AHEAD) load_values(here, 0);
+            for (;; u += 4) {
+            const bool more = u + 4 < u1;
+            if (more) next.find(p, table, rq.len, u + 4, h, W, lane);
+            // (a unit without a block is masked altogether: a branch round the arithmetic costs more registers than the kernel has)
+            const bool boundary = 64 * u + 64 > st.limit_min || here.none;
+            {
+                const int key0 = 64 * u + 16 * lg;
+                f32x4 s[NR][4];
+                typename State::vec8 w[NR][2];
+                st.scores([&](int t, int c) { return fragment<T>(kr[t][c >> 1][2 * (c & 1)], kr[t][c >> 1][2 * (c & 1) + 1]); }, s);
+                if (!AHEAD) load_values(here, 0);
+                else if (more) load_keys(next);
+                else drop_keys();
+                st.template softmax<SMALL>(s, w, key0, here.kf, here.dead, here.ratio, boundary);
+                bool nan = false;
+                const auto part = [&](auto from) {
+                    constexpr int D0 = decltype(from)::value;
+                    if (64 * u + 64 > rq.len || __any(here.dead)) {
+                        const int valid = here.dead ? 0 : rq.len - key0;
+#pragma unroll
+                        for (int d = 0; d < VN; ++d) vr[d] = clear_behind(vr[d], valid);
+                    }
+                    if (boundary) {
+                        const int slot = fresh_lane(4 * wk + lg);       // the lane's place in nan_keys[wave], 64 apart for each column tile
+                        unsigned short* keys = nan_keys[wave] + slot;
+                        bool mine = false;
+#pragma unroll
+                        for (int d = 0; d < VN; ++d) mine |= has_nan(vr[d]);
+                        if (!nan && __any(mine)) {
+                            nan = true;
+                            for (int d = 0; d < ND; ++d) keys[64 * d] = 0;
+                        }
+                        if (nan) {
+#pragma unroll
+                            for (int d = 0; d < VN; ++d) {
+                                keys[64 * (D0 + d)] = (unsigned short)take_nan(vr[d]);
+                                __builtin_amdgcn_sched_barrier(0);
+                            }
+                        }
+                    }
+                    st.template values<D0, D0 + VN>([&](int d, int v) { return fragment<T>(vr[d - D0][2 * v], vr[d - D0][2 * v + 1]); }, w, here.vs);
+                };
+                fa_static_for<0, ND / VN>([&](auto i) {
+                    if constexpr (decltype(i)::value > 0) load_values(here, decltype(i)::value * VN);
+                    part(std::integral_constant<int, decltype(i)::value * VN>{});
+                });
+                if (nan) st.note_nan((const unsigned long long*)nan_keys[wave], u, lg);
+            }
+            if (!more) break;
+            if (AHEAD) load_values(next, 0);
+            else load_keys(next);
+            here = next;
+            }
+        }
+        // the waves' parts joined, the first wave ends with the sums
+        const int active = min(4, u1 - u0);
+        st.put_nan();
+    float sum[NR], top[NR];
+#pragma unroll
+        for (int r = 0; r < NR; ++r) { sum[r] = rows_sum(st.l[r]); top[r] = st.m[r]; }
+        if (active > 1) {
+            if (lg == 0) {
+#pragma unroll
+                for (int r = 0; r < NR; ++r) { join_m[wave][16 * r + wk] = top[r]; join_l[wave][16 * r + wk] = sum[r]; }
+            }
+            __syncthreads();
+#pragma unroll
+            for (int r = 0; r < NR; ++r) {
+                float all = -INFINITY, total = 0.f;
+#pragma unroll
+                for (int w = 0; w < 4; ++w) all = __builtin_fmaxf(all, join_m[w][16 * r + wk]);
+                const float base = all == -INFINITY ? 0.f : all;
+#pragma unroll
+                for (int w = 0; w < 4; ++w) total += join_l[w][16 * r + wk] * fast_exp2(join_m[w][16 * r + wk] - base);
+                const float f = fast_exp2(top[r] - base);
+#pragma unroll
+                for (int d = 0; d < ND; ++d)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) st.o[r][d][i] *= f;
+                top[r] = all;
+                sum[r] = total;
+            }
+#pragma unroll
+            for (int step = 2; step >= 1; step >>= 1) {
+                if (wave >= step && wave < 2 * step) {
+#pragma unroll
+                    for (int r = 0; r < NR; ++r)
+#pragma unroll
+                        for (int d = 0; d < ND; ++d) join_o[wave - step][(r * ND + d) * 64 + lane] = f32x4{st.o[r][d][0], st.o[r][d][1], st.o[r][d][2], st.o[r][d][3]};
+                }
+                __syncthreads();
+                if (wave < step) {
+#pragma unroll
+                    for (int r = 0; r < NR; ++r)
+#pragma unroll
+                        for (int d = 0; d < ND; ++d) {
+                            const f32x4 v = join_o[wave][(r * ND + d) * 64 + lane];
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) st.o[r][d][i] += v[i];
+                        }
+                }
+                __syncthreads();
+            }
+        }
+        if (wave == 0) {
+            if (whole) st.store(p, rq, h, row0, lane, sum);
+            else st.park(p, 2ll * blockIdx.x + (cur == start ? 0 : 1), ROWS, 0, lane, sum, top);
+        }
+        cur += u1 - u0;
+        off += u1 - u0;
+    }
+}
+
+// query tiles of 16 rows per wave: two where O (16 NR W / 64 registers) leaves room for two waves per SIMD
+constexpr int tile_nr(int W) { return W <= 128 ? 2 : 1; }
+
+// ---- tile kernel --------------------------------------------------------------------------------------------------------------------------
+template <typename T, int W, bool SMALL>
+__global__ __launch_bounds__(256, W > 128 ? 1 : 2) void cache_tile_kernel(CacheAttnParams p) {
+    constexpr int NR = tile_nr(W), ROWS = 64 * NR, NK = W / 64, ND = W / 16, NC = W / 32, KPW = NK, VPW = ND / 4;
+    using State = RowState<T, W, NR>;
+    using vec8 = typename State::vec8;
+    __shared__ u32x4 lds_k[2][4 * NC * 64], lds_v[2][2 * ND * 64];
+    __shared__ __align__(8) unsigned short nan_keys[2][4 * W];     // [buffer][column][16-key group]
+    __shared__ int nan_found[2];
+    const int lane = (int)threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+    const int lg = lane >> 4, wk = lane & 15;
+    // block -> (head, part, tile): the head is the fastest, so that the tiles that share codes run on one XCD where the head count divides 8
+    // or is a multiple of it; late tiles (the long ones of a prompt) first
+    const int idx = (int)blockIdx.x, h = idx % p.Hkv, rest = idx / p.Hkv, part = rest % p.splits, order = rest / p.splits;
+    long long tile = 0;
+    const Place at = find_place<256>(p.B, [&](int b) { return (long long)((request_of(p, b).n * p.group + ROWS - 1) / ROWS); },
+                                     [&](long long total) { tile = total - 1 - order; return tile; }, blockIdx.x == 0 ? p.ws_prefix : nullptr);
+    if (order >= at.total || tile >= p.max_tiles) return;      // (more tiles than tokens allow: cu_q is not ascending)
+    const Request rq = request_of(p, at.b);
+    const int row0 = (int)at.off * ROWS;
+    const int* table = p.tables + (int64_t)at.b * p.table_stride;
+    State st;
+    st.load(p, rq, h, row0 + 16 * NR * wave, lane);
+    st.clear();
+    const int last = min(row0 + ROWS, rq.n * p.group) - 1;
+    const int see = rq.len - rq.n + last / p.group + 1;            // keys that the tile's last row sees
+    const int units = see > 0 ? (see + 63) >> 6 : 0;
+    const int u0 = (int)((long long)units * part / p.splits), u1 = (int)((long long)units * (part + 1) / p.splits);
+    const bool idle = row0 + 16 * NR * wave > last;                     // (a wave without rows still brings its share of the operands)
+
+    const int tile_min = rq.len - rq.n + row0 / p.group + 1;        // keys that its first row sees
+    if (threadIdx.x < 2) nan_found[threadIdx.x] = 0;
+    __syncthreads();
+
+    // operands of a unit: wave w brings key tile w and the value columns of ND / 4 tiles
+    u32x4 kr[KPW], vr[VPW];
+    UnitAt<SMALL> here, next;
+    const unsigned key_off = UnitAt<SMALL>::key_lane(W, lane), value_off = UnitAt<SMALL>::value_lane(p.shift, lane);
+    const auto load = [&](const UnitAt<SMALL>& a) {
+#pragma unroll
+        for (int i = 0; i < KPW; ++i) kr[i] = *(const u32x4*)(a.k + (4 * wave * W + 64 * i) + key_off);
+#pragma unroll
+        for (int i = 0; i < VPW; ++i) vr[i] = *(const u32x4*)(a.v + ((16 * (wave * VPW + i)) << p.shift) + value_off);
+    };
+    const auto spread = [&](const UnitAt<SMALL>& a, int u, int buf) {
+#pragma unroll
+        for (int i = 0; i < KPW; ++i)
+#pragma unroll
+            for (int c = 0; c < 2; ++c)
+                lds_k[buf][(wave * NC + 2 * i + c) * 64 + lane] = __builtin_bit_cast(u32x4, fragment<T>(kr[i][2 * c], kr[i][2 * c + 1]));
+        if (64 * u + 64 > rq.len || (SMALL && __any(a.dead))) {
+            const int valid = a.dead ? 0 : rq.len - (64 * u + 16 * lg);
+#pragma unroll
+            for (int i = 0; i < VPW; ++i) vr[i] = clear_behind(vr[i], valid);
+        }
+        if (64 * u + 64 > tile_min) {                               // (uniform) a unit that some rows see in part
+            bool mine = false;
+#pragma unroll
+            for (int i = 0; i < VPW; ++i) {
+                mine |= has_nan(vr[i]);
+                nan_keys[buf][64 * (wave * VPW + i) + 4 * wk + lg] = (unsigned short)take_nan(vr[i]);
+            }
+            if (mine) nan_found[buf] = u + 1;                       // (no other value is written here: a unit's mark is its own number)
+        }
+#pragma unroll
+        for (int i = 0; i < VPW; ++i)
+#pragma unroll
+            for (int c = 0; c < 2; ++c)
+                lds_v[buf][((wave * VPW + i) * 2 + c) * 64 + lane] = __builtin_bit_cast(u32x4, fragment<T>(vr[i][2 * c], vr[i][2 * c + 1]));
+    };
+    if (u0 < u1) {
+        here.find(p, table, rq.len, u0, h, W, lane);
+        load(here);
+        spread(here, u0, 0);
+    }
+    __syncthreads();
+    for (int u = u0; u < u1; ++u) {
+        const int buf = (u - u0) & 1;
+        const bool more = u + 1 < u1;
+        if (more) {
+            next.find(p, table, rq.len, u + 1, h, W, lane);
+            load(next);
+        }
+        if (!here.none && !idle && 64 * u < st.limit_max) {
+            const int key0 = 64 * u + 16 * lg;
+            const bool boundary = 64 * u + 64 > st.limit_min;
+            f32x4 s[NR][4];
+            vec8 w[NR][2];
+            st.scores([&](int t, int c) { return __builtin_bit_cast(vec8, lds_k[buf][(t * NC + c) * 64 + lane]); }, s);
+            st.template softmax<SMALL>(s, w, key0, here.kf, here.dead, here.ratio, boundary);
+            st.template values<0, ND>([&](int d, int v) { return __builtin_bit_cast(vec8, lds_v[buf][(d * 2 + v) * 64 + lane]); }, w, here.vs);
+            if (nan_found[buf] == u + 1) st.note_nan((const unsigned long long*)nan_keys[buf], u, lg);
+        }
+        if (more) {
+            spread(next, u + 1, buf ^ 1);
+            here = next;
+        }
+        __syncthreads();
+    }
+    st.put_nan();
+    float sum[NR], top[NR];
+#pragma unroll
+    for (int r = 0; r < NR; ++r) { sum[r] = rows_sum(st.l[r]); top[r] = st.m[r]; }
+    if (p.splits == 1) st.store(p, rq, h, row0 + 16 * NR * wave, lane, sum);
+    else st.park(p, ((long long)h * p.max_tiles + tile) * p.splits + part, ROWS, 16 * NR * wave, lane, sum, top);
+}
+
+// ---- join kernel: partial sums of one (request, key/value head, row tile), 64 columns per workgroup -------------------------------------------
+// slots in order, so that results are the same from call to call
+template <typename T, bool TILE>
+__global__ __launch_bounds__(256) void cache_join_kernel(CacheAttnParams p, int W, int rows16) {
+    __shared__ f32x4 part_o[256];
+    __shared__ float part_m[256], part_l[256];
+    int b, h, tile;
+    long long item0 = 0, range = 1, w0, w1, slot0 = 0;
+    if constexpr (TILE) {
+        h = (int)blockIdx.x % p.Hkv;
+        const long long t = (int)blockIdx.x / p.Hkv;
+        if (t >= p.ws_prefix[p.B] || t >= p.max_tiles) return;
+        int lo = 0, hi = p.B;
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) >> 1;
+            if (p.ws_prefix[mid] <= t) lo = mid; else hi = mid;
+        }
+        b = lo;
+        tile = (int)(t - p.ws_prefix[b]);
+        w0 = 0;
+        w1 = p.splits - 1;
+        slot0 = ((long long)h * p.max_tiles + t) * p.splits;
+    } else {
+        b = (int)blockIdx.x / p.Hkv;
+        h = (int)blockIdx.x - b * p.Hkv;
+        tile = (int)blockIdx.y;
+    }
+    const Request rq = request_of(p, b);
+    const int rows = rq.n * p.group, tiles = (rows + rows16 - 1) / rows16, tid = (int)threadIdx.x;
+    for (; tile < tiles; tile += TILE ? tiles : (int)gridDim.y) {      // (more row tiles than the grid was told: every one is still reached)
+        if constexpr (!TILE) {
+            range = range_of(p, p.ws_prefix[p.B]);
+            item0 = p.ws_prefix[b] + ((long long)h * tiles + tile) * rq.units;
+            w0 = item0 / range;
+            w1 = (item0 + rq.units - 1) / range;
+            if (w0 == w1) continue;                                    // (finished by one workgroup)
+        }
+        // threads: strands of slots x rows x 16 groups of four columns
+        for (int base = 0; base < min(rows16, rows - tile * rows16); base += 16) {
+            const int live = min(16, rows - tile * rows16 - base);
+            const int lanes = live > 8 ? 256 : live > 4 ? 128 : live > 2 ? 64 : live > 1 ? 32 : 16;
+            const int strands = 256 / lanes, strand = tid / lanes, row = (tid % lanes) >> 4, c = tid & 15;
+            const int col = 64 * (int)blockIdx.z + 4 * c;
+            float top = -INFINITY, sum = 0.f;
+            f32x4 o = {0.f, 0.f, 0.f, 0.f};
+            if (row < live) {
+                for (long long w = w0 + strand; w <= w1; w += strands) {
+                    const long long slot = TILE ? slot0 + w : 2 * w + (w * range >= item0 ? 0 : 1);
+                    const long long at = slot * rows16 + base + row;
+                    const float m = p.ws_ml[2 * at], l = p.ws_ml[2 * at + 1];
+                    const f32x4 v = *(const f32x4*)(p.ws_o + at * W + col);
+                    const float now = __builtin_fmaxf(top, m), b0 = now == -INFINITY ? 0.f : now;
+                    const float f0 = fast_exp2(top - b0), f1 = fast_exp2(m - b0);
+                    o = o * f0 + v * f1;
+                    sum = sum * f0 + l * f1;
+                    top = now;
+                }
+            }
+            part_o[tid] = o;
+            part_m[tid] = top;
+            part_l[tid] = sum;
+            __syncthreads();
+            if (strand == 0 && row < live) {
+                for (int s = 1; s < strands; ++s) {
+                    const int i = s * lanes + tid;
+                    const float m = part_m[i], now = __builtin_fmaxf(top, m), b0 = now == -INFINITY ? 0.f : now;
+                    const float f0 = fast_exp2(top - b0), f1 = fast_exp2(m - b0);
+                    o = o * f0 + part_o[i] * f1;
+                    sum = sum * f0 + part_l[i] * f1;
+                    top = now;
+                }
+                const float inv = sum == 0.f ? 0.f : 1.0f / sum;
+                const int r = tile * rows16 + base + row, i = r / p.group, g = r - i * p.group;
+                if (col < p.D) {
+                    o *= inv;
+                    T* dst = (T*)p.o + (int64_t)(rq.first + i) * p.o_st + (int64_t)(h * p.group + g) * p.o_sh + col;
+                    *(u32x2c*)dst = u32x2c{pack2<T>(o[0], o[1]), pack2<T>(o[2], o[3])};
+                }
+            }
+            __syncthreads();
+        }
+    }
+}
+
+template <typename T, int W>
+hipError_t launch_width(const CacheAttnParams& p, const CacheAttnPlan& plan, hipStream_t stream) {
+    const bool small = p.shift < 6;
+    const void* k;
+    if (plan.tile) k = small ? (const void*)cache_tile_kernel<T, W, true> : (const void*)cache_tile_kernel<T, W, false>;
+    else if (W > 128 || plan.nr == 1) k = small ? (const void*)cache_rows_kernel<T, W, 1, true> : (const void*)cache_rows_kernel<T, W, 1, false>;
+    else k = small ? (const void*)cache_rows_kernel<T, W <= 128 ? W : 128, 2, true> : (const void*)cache_rows_kernel<T, W <= 128 ? W : 128, 2, false>;
+    return launch1(k, dim3((unsigned)plan.grid), dim3(256), 0, stream, p);
+}
+template <typename T>
+hipError_t launch_typed(const CacheAttnParams& p, const CacheAttnPlan& plan, hipStream_t stream) {
+    hipError_t e = plan.width == 64 ? launch_width<T, 64>(p, plan, stream) : plan.width == 128 ? launch_width<T, 128>(p, plan, stream)
+                 : plan.width == 192 ? launch_width<T, 192>(p, plan, stream) : launch_width<T, 256>(p, plan, stream);
+    if (e != hipSuccess || (plan.tile && plan.splits == 1)) return e;
+    const int rows16 = (plan.tile ? 64 : 16) * plan.nr;
+    CacheAttnParams arg = p;
+    int W = plan.width, rows = rows16;
+    void* args[] = {&arg, &W, &rows};
+    const dim3 grid((unsigned)(p.Hkv * (plan.tile ? plan.max_tiles : p.B)), plan.tile ? 1u : (unsigned)plan.max_tiles, (unsigned)(plan.width / 64));
+    return hipLaunchKernel(plan.tile ? (const void*)cache_join_kernel<T, true> : (const void*)cache_join_kernel<T, false>, grid, dim3(256), args, 0, stream);
+}
+
+}  // namespace
+
+hipError_t launch_cache_attn(const CacheAttnParams& p, const CacheAttnPlan& plan, int dtype, hipStream_t stream) {
+    return dtype == 0 ? launch_typed<_Float16>(p, plan, stream) : launch_typed<__bf16>(p, plan, stream);
+}
+
+}  // namespace fa

@@ -1,0 +1,412 @@
+// What changes the state of a block cache: block tables and slots of a step, and new keys and values as e4m3 codes.
+#include <hip/hip_runtime.h>
+
+#include "fa_cache.h"
+#include "fa_params.h"
+
+namespace fa {
+namespace {
+
+// ---- block tables, positions, slots ------------------------------------------------------------------------------------------------------
+// Requests b = 0 .. B-1 hold held[b] tokens in ceil(held / P) blocks; n[b] tokens come (n < 0: the request ends).
+//   1. the blocks of the requests that end are put behind the free ones, in the order of the requests and of their blocks;
+//   2. cu = running sum of max(n, 0); a request fits if cu[b+1] <= T and its blocks fit the table; its need is the number of blocks to add;
+//      it is served if it fits and needs nothing or the needs of all that fit up to and including it are there;
+//   3. blocks are taken from the end of the free list, in the order of the requests; positions and slots follow.
+// Bound: latency - a few kilobytes through one workgroup, three scans.  Sums saturate at 2^31 - 1 (which stays associative, so that the
+// scan order does not matter) where lengths add up to more.
+constexpr int kScanThreads = 1024;
+
+__device__ __forceinline__ int sat_add(int a, int b) {
+    const unsigned s = (unsigned)a + (unsigned)b;
+    return s > 0x7fffffffu ? 0x7fffffff : (int)s;
+}
+// exclusive scan over the workgroup with saturation; `total` is every thread's
+__device__ __forceinline__ int block_scan(int x, int* waves, int& total) {
+    const int lane = (int)threadIdx.x & 63, wave = (int)threadIdx.x >> 6;
+    int incl = x;
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) {
+        const int y = __shfl_up(incl, d);
+        if (lane >= d) incl = sat_add(incl, y);
+    }
+    if (lane == 63) waves[wave] = incl;
+    __syncthreads();
+    int before = 0;
+    total = 0;
+#pragma unroll
+    for (int w = 0; w < kScanThreads / 64; ++w) {
+        if (w == wave) before = total;
+        total = sat_add(total, waves[w]);
+    }
+    __syncthreads();
+    const int prev = __shfl_up(incl, 1);
+    return sat_add(before, lane ? prev : 0);
+}
+// largest i in [0, n) with first[i] <= x; first is ascending, first[0] <= x
+__device__ __forceinline__ int find(const int* first, int n, int x) {
+    int lo = 0, hi = n;
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (first[mid] <= x) lo = mid; else hi = mid;
+    }
+    return lo;
+}
+__device__ __forceinline__ int blocks_of(int64_t tokens, int shift) { return (int)((tokens + (1 << shift) - 1) >> shift); }
+
+// position and slot of token t of request b, which starts at `start` and has `granted` of its tokens granted (all or none) and `total` held then
+__device__ __forceinline__ void place(const TablesParams& p, int t, int b, int start, int granted, int total) {
+    int pos = -1, slot = -1;
+    if (granted > 0) {
+        pos = total - granted + (t - start);
+        const int block = p.tables[(int64_t)b * p.table_stride + (pos >> p.shift)];
+        if (block >= 0) slot = (block << p.shift) + (pos & ((1 << p.shift) - 1));
+    }
+    p.positions[t] = pos;
+    p.slots[t] = slot;
+}
+
+__global__ __launch_bounds__(kScanThreads) void cache_tables_kernel(TablesParams p) {
+    __shared__ int waves[kScanThreads / 64], first[kScanThreads], start[kScanThreads], have_s[kScanThreads];
+    const int tid = (int)threadIdx.x;
+    int free = *p.free_in;
+    free = free < 0 ? 0 : free > p.pool_size ? p.pool_size : free;
+    // 1. ended requests' blocks
+    for (int base = 0; base < p.B; base += kScanThreads) {
+        const int b = base + tid;
+        const bool ends = b < p.B && p.new_lens[b] < 0;
+        const int held = ends ? max(p.seq_in[b], 0) : 0;
+        const int back = ends ? min(blocks_of(held, p.shift), p.width) : 0;
+        int total;
+        const int at = block_scan(back, waves, total);
+        if (total > 0) {                       // (uniform)
+            first[tid] = at;
+            __syncthreads();
+            for (int i = tid; i < total; i += kScanThreads) {
+                const int r = find(first, kScanThreads, i), to = sat_add(free, i);
+                if (to < p.pool_size) p.pool[to] = p.tables[(int64_t)(base + r) * p.table_stride + (i - first[r])];
+            }
+            __syncthreads();
+        }
+        free = min(sat_add(free, total), p.pool_size);
+    }
+    // 2. and 3.
+    int tokens = 0, needed = 0, taken = 0;     // running sums over the chunks of requests
+    for (int base = 0; base < p.B; base += kScanThreads) {
+        const int b = base + tid;
+        const bool in = b < p.B;
+        const int n = in ? p.new_lens[b] : 0, count = max(n, 0), held = in ? max(p.seq_in[b], 0) : 0;
+        int total;
+        const int my_start = sat_add(tokens, block_scan(count, waves, total)), my_end = sat_add(my_start, count);
+        tokens = sat_add(tokens, total);
+        const int have = blocks_of(held, p.shift);
+        const int64_t after = ((int64_t)held + count + (1 << p.shift) - 1) >> p.shift;
+        const bool fits = in && n >= 0 && after <= p.width && my_end <= p.T;
+        const int need = fits ? (int)after - have : 0;
+        const int before = sat_add(needed, block_scan(need, waves, total));
+        needed = sat_add(needed, total);
+        const bool served = fits && (need == 0 || sat_add(before, need) <= free);
+        const int granted = served ? count : 0;
+        const int add = served ? need : 0;
+        const int my_first = sat_add(taken, block_scan(add, waves, total));
+        if (total > 0) {                       // (uniform)
+            first[tid] = my_first;
+            have_s[tid] = have;
+            __syncthreads();
+            for (int i = tid; i < total; i += kScanThreads) {
+                const int k = taken + i, r = find(first, kScanThreads, k);
+                p.tables[(int64_t)(base + r) * p.table_stride + have_s[r] + (k - first[r])] = p.pool[free - 1 - k];
+            }
+            __syncthreads();
+        }
+        taken += total;
+        const int held_after = n < 0 ? 0 : held + granted;
+        if (in) {
+            p.seq_out[b] = held_after;
+            p.granted[b] = granted;
+            p.cu_new[b] = my_start;
+            if (b == p.B - 1) p.cu_new[p.B] = my_end;
+        }
+        if (p.fused) {
+            // the tokens of this chunk of requests; first / start / have_s serve as request starts, grants and lengths
+            first[tid] = my_start;
+            start[tid] = granted;
+            have_s[tid] = held_after;
+            __syncthreads();
+            const int from = base == 0 ? 0 : first[0], to = min(tokens, p.T);
+            for (int t = from + tid; t < to; t += kScanThreads) {
+                const int r = find(first, min(p.B - base, kScanThreads), t);
+                place(p, t, base + r, first[r], start[r], have_s[r]);
+            }
+            __syncthreads();
+        }
+    }
+    if (p.fused)
+        for (int t = min(tokens, p.T) + tid; t < p.T; t += kScanThreads) p.positions[t] = p.slots[t] = -1;
+    if (tid == 0) *p.free_out = free - taken;
+}
+
+constexpr int kSlotThreads = 256, kSlotStage = 2048;
+__global__ __launch_bounds__(kSlotThreads) void cache_slots_kernel(TablesParams p) {
+    __shared__ int staged[kSlotStage];
+    const int t = (int)blockIdx.x * kSlotThreads + (int)threadIdx.x;
+    const int* first = p.cu_new;
+    if (p.B <= kSlotStage) {                   // (B + 1 entries; the last one bounds the tokens and is read from memory)
+        for (int i = (int)threadIdx.x; i < p.B; i += kSlotThreads) staged[i] = p.cu_new[i];
+        __syncthreads();
+        first = staged;
+    }
+    if (t >= p.T) return;
+    if (t >= p.cu_new[p.B]) {
+        p.positions[t] = p.slots[t] = -1;
+        return;
+    }
+    const int b = find(first, p.B, t);
+    place(p, t, b, first[b], p.granted[b], p.seq_out[b]);
+}
+
+// ---- new keys and values -----------------------------------------------------------------------------------------------------------------
+// A run is a stretch of tokens whose slots follow each other inside one block.  For a run, a head and one of the two caches:
+//   A = largest finite |x|;  wanted = 2^e, the smallest power of two with A <= 448 * 2^e (e >= -100);
+//   a run that begins its block sets the scale to `wanted`; any other run raises it to max(scale, wanted), and where that changes it every
+//   code of the block is brought to the new scale;  codes = nearest e4m3 of x / scale (ties to even); inf and NaN become the code of NaN.
+// Scales are powers of two because codes carry their own exponent: x / scale is exact, growing a scale only moves the codes' exponents (exact
+// but for what falls under the smallest code), and nothing is gained by filling the last fraction of the top binade.
+// Bound: memory (2 bytes in, 1 byte out per value) for prompts, latency for a step.  A workgroup owns `window` tokens of one head and cache;
+// the runs that begin in them are its work - a run is never shared, so scales need no atomics.  Long runs are taken by the whole workgroup,
+// several short ones by a wave each.
+// A work item is eight columns of four consecutive tokens: 16-byte loads, the values stay in registers between the maximum and the codes, and
+// both layouts store whole words - eight bytes of a key row, or (columns down the lanes) four tokens of a value column.
+template <typename T> struct Bits;
+template <> struct Bits<_Float16> {
+    static constexpr unsigned top = 0x7c00u;
+    static __device__ __forceinline__ float f(unsigned u) { return (float)__builtin_bit_cast(_Float16, (unsigned short)u); }
+};
+template <> struct Bits<__bf16> {
+    static constexpr unsigned top = 0x7f80u;
+    static __device__ __forceinline__ float f(unsigned u) { return __builtin_bit_cast(float, u << 16); }
+};
+
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
+typedef unsigned u32x4v __attribute__((ext_vector_type(4)));
+
+// |x| <= 448 by the choice of the scale, except inf and NaN, which become the code of NaN
+__device__ __forceinline__ unsigned codes2(float a, float b) {
+    const float inf = __builtin_inff();
+    a = __builtin_fabsf(a) == inf ? __builtin_nanf("") : a;
+    b = __builtin_fabsf(b) == inf ? __builtin_nanf("") : b;
+    return (unsigned)__builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false) & 0xffffu;
+}
+__device__ __forceinline__ unsigned rescale4(unsigned w, float f) {
+    const f32x2 lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, false), hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, true);
+    return codes2(lo[0] * f, lo[1] * f) | codes2(hi[0] * f, hi[1] * f) << 16;
+}
+__device__ __forceinline__ float wanted_scale(float largest) {
+    const unsigned u = __builtin_bit_cast(unsigned, largest);
+    int e = (int)(u >> 23) - 126 - 9 + ((u & 0x7fffffu) > 0x600000u);    // largest = m 2^E, m in [0.5, 1): e = E - 9 + (m > 0.875)
+    e = e < -100 ? -100 : e;
+    return __builtin_bit_cast(float, (unsigned)(e + 127) << 23);
+}
+__device__ __forceinline__ unsigned wave_max(unsigned x) {
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) {
+        const unsigned y = (unsigned)__shfl_xor((int)x, d);
+        x = x > y ? x : y;
+    }
+    return x;
+}
+
+// one run: tokens t0 .. t0 + n - 1 into positions off .. off + n - 1 of a block.  NT = 64 (a wave) or 256 (the workgroup)
+template <typename T, bool KEYS, int NT>
+__device__ __forceinline__ void append_run(const AppendParams& p, int t0, int n, int64_t block, int off, int head, unsigned* shared_max) {
+    const int tid = (int)threadIdx.x & (NT - 1);
+    const int P = 1 << p.shift, W = p.W, chunks = p.D >> 3, wchunks = W >> 3;
+    const int g0 = off >> 2, groups = ((off + n + 3) >> 2) - g0;          // groups of four positions that the run touches
+    const T* x = (const T*)p.x[KEYS ? 0 : 1] + (int64_t)head * p.x_sh[KEYS ? 0 : 1];
+    const int64_t st = p.x_st[KEYS ? 0 : 1];
+    uint8_t* tile = (uint8_t*)p.cache[KEYS ? 0 : 1] + block * p.block_stride[KEYS ? 0 : 1] + (int64_t)head * P * W;
+    float* scale = p.scale[KEYS ? 0 : 1] + block * p.scale_stride[KEYS ? 0 : 1] + head;
+    const float old = off ? *scale : 0.f;
+
+    const auto load = [&](int i, u32x4v (&v)[4], int& g, int& c) {        // item i: position group g, column chunk c
+        if (KEYS) { g = g0 + i / wchunks; c = i % wchunks; }
+        else { g = g0 + i % groups; c = i / groups; }
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const int k = 4 * g + r - off;
+            if (k >= 0 && k < n && c < chunks) v[r] = *(const u32x4v*)(x + (int64_t)(t0 + k) * st + 8 * c);
+            else v[r] = u32x4v{0, 0, 0, 0};
+        }
+    };
+    const int items = groups * wchunks;
+    constexpr int HOLD = 2;                    // items per thread that stay in registers between the two passes
+    u32x4v held[HOLD][4];
+    unsigned largest = 0;
+    const auto look = [&](const u32x4v (&v)[4]) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const unsigned lo = v[r][q] & 0x7fffu, hi = (v[r][q] >> 16) & 0x7fffu;
+                if (lo < Bits<T>::top && lo > largest) largest = lo;
+                if (hi < Bits<T>::top && hi > largest) largest = hi;
+            }
+    };
+    int g, c;
+#pragma unroll
+    for (int h = 0; h < HOLD; ++h)
+        if (tid + h * NT < items) { load(tid + h * NT, held[h], g, c); look(held[h]); }
+    for (int i = tid + HOLD * NT; i < items; i += NT) {
+        u32x4v v[4];
+        load(i, v, g, c);
+        look(v);
+    }
+    largest = wave_max(largest);
+    if constexpr (NT == 256) {
+        if ((threadIdx.x & 63) == 0) shared_max[threadIdx.x >> 6] = largest;
+        __syncthreads();
+        largest = max(max(shared_max[0], shared_max[1]), max(shared_max[2], shared_max[3]));
+    }
+    const float wanted = wanted_scale(Bits<T>::f(largest));
+    const float now = off == 0 ? wanted : old > wanted ? old : wanted;
+    if (off != 0 && now != old) {              // (uniform over the NT threads)
+        const float f = old / now;
+        for (int i = tid; i < P * W / 16; i += NT) {
+            u32x4v w = *(const u32x4v*)(tile + 16 * i);
+#pragma unroll
+            for (int q = 0; q < 4; ++q) w[q] = rescale4(w[q], f);
+            *(u32x4v*)(tile + 16 * i) = w;
+        }
+        __threadfence();                       // these stores are done before the run's own bytes are written
+    }
+    if constexpr (NT == 256) __syncthreads();  // everyone has read the old scale, the rescaled block is written
+    if (tid == 0) *scale = now;
+    const float inv = __builtin_bit_cast(float, (254u << 23) - __builtin_bit_cast(unsigned, now));   // 1 / 2^e
+    const bool pow2 = (__builtin_bit_cast(unsigned, now) & 0x807fffffu) == 0u && now < 0x1p126f;
+    const auto put = [&](int i, const u32x4v (&v)[4]) {
+        int gg, cc;
+        if (KEYS) { gg = g0 + i / wchunks; cc = i % wchunks; }
+        else { gg = g0 + i % groups; cc = i / groups; }
+        u32x2 code[4];                         // row r: eight columns
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+#pragma unroll
+            for (int q = 0; q < 2; ++q) {
+                unsigned w = 0;
+#pragma unroll
+                for (int z = 0; z < 2; ++z) {
+                    const unsigned u = v[r][2 * q + z];
+                    const float a = Bits<T>::f(u & 0xffffu), b = Bits<T>::f(u >> 16);
+                    w |= (pow2 ? codes2(a * inv, b * inv) : codes2(a / now, b / now)) << (16 * z);
+                }
+                code[r][q] = w;
+            }
+        }
+        const int first = 4 * gg - off;        // run index of the group's first position
+        if (KEYS) {
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+                if (first + r >= 0 && first + r < n) *(u32x2*)(tile + (4 * gg + r) * W + 8 * cc) = code[r];
+        } else {
+            const bool whole = first >= 0 && first + 4 <= n;
+#pragma unroll
+            for (int col = 0; col < 8; ++col) {
+                const int q = col >> 2, b = (col & 3) * 8;
+                const unsigned w = ((code[0][q] >> b) & 0xffu) | ((code[1][q] >> b) & 0xffu) << 8 | ((code[2][q] >> b) & 0xffu) << 16 |
+                                   ((code[3][q] >> b) & 0xffu) << 24;
+                uint8_t* to = tile + (8 * cc + col) * P + 4 * gg;
+                if (whole) *(unsigned*)to = w;
+                else {
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+                        if (first + r >= 0 && first + r < n) to[r] = (uint8_t)(w >> (8 * r));
+                }
+            }
+        }
+    };
+#pragma unroll
+    for (int h = 0; h < HOLD; ++h)
+        if (tid + h * NT < items) put(tid + h * NT, held[h]);
+    for (int i = tid + HOLD * NT; i < items; i += NT) {
+        u32x4v v[4];
+        load(i, v, g, c);
+        put(i, v);
+    }
+    if constexpr (NT == 256) __syncthreads();  // shared_max is free again
+}
+
+template <typename T>
+__global__ __launch_bounds__(256) void cache_append_kernel(AppendParams p) {
+    __shared__ int run_first[64], run_len[64], run_count;
+    __shared__ unsigned shared_max[4];
+    const int lane = (int)threadIdx.x & 63, wave = (int)threadIdx.x >> 6;
+    const int head = (int)blockIdx.y >> 1;
+    const bool keys = ((int)blockIdx.y & 1) == 0;
+    const int P = 1 << p.shift, t_first = (int)blockIdx.x * p.window;
+    // the runs that begin in the window: a token begins one unless its slot follows its predecessor's inside a block
+    if (wave == 0) {
+        const int t = t_first + lane;
+        int slot = -1;
+        bool begins = false;
+        if (lane < p.window && t < p.T) {
+            slot = p.slots[t];
+            if (slot >= 0 && slot < p.limit) {
+                const int prev = t ? p.slots[t - 1] : -2;
+                begins = prev < 0 || prev + 1 != slot || (slot & (P - 1)) == 0;
+            }
+        }
+        const unsigned long long m = __ballot(begins);
+        if (begins) run_first[__popcll(m & ((1ull << lane) - 1))] = t;
+        if (lane == 0) run_count = __popcll(m);
+    }
+    __syncthreads();
+    const int runs = run_count;
+    if (runs == 0) return;
+    // their lengths: up to the end of the block
+    for (int r = wave; r < runs; r += 4) {
+        const int t0 = run_first[r], slot = p.slots[t0], room = P - (slot & (P - 1));
+        int n = 0;
+        for (int at = 0; at < room; at += 64) {
+            const int k = at + lane;
+            const bool same = k < room && t0 + k < p.T && p.slots[t0 + k] == slot + k;
+            const unsigned long long m = __ballot(same);
+            const int ones = ~m ? __builtin_ctzll(~m) : 64;
+            n += ones;
+            if (ones < 64) break;
+        }
+        if (lane == 0) run_len[r] = n;
+    }
+    __syncthreads();
+    // one or two runs in a window of 16 tokens and more are long: the whole workgroup; else a wave per run
+    const bool together = p.window >= 16 && runs <= 2;
+    for (int r = together ? 0 : wave; r < runs; r += together ? 1 : 4) {
+        const int t0 = __builtin_amdgcn_readfirstlane(run_first[r]), n = __builtin_amdgcn_readfirstlane(run_len[r]);
+        const int slot = __builtin_amdgcn_readfirstlane(p.slots[t0]);
+        const int64_t block = slot >> p.shift;
+        const int off = slot & (P - 1);
+        if (together) {
+            if (keys) append_run<T, true, 256>(p, t0, n, block, off, head, shared_max);
+            else append_run<T, false, 256>(p, t0, n, block, off, head, shared_max);
+        } else {
+            if (keys) append_run<T, true, 64>(p, t0, n, block, off, head, shared_max);
+            else append_run<T, false, 64>(p, t0, n, block, off, head, shared_max);
+        }
+    }
+}
+
+}  // namespace
+
+hipError_t launch_cache_tables(const TablesParams& p, hipStream_t stream) {
+    hipError_t e = launch1((const void*)cache_tables_kernel, dim3(1), dim3(kScanThreads), 0, stream, p);
+    if (e == hipSuccess && !p.fused && p.T > 0)
+        e = launch1((const void*)cache_slots_kernel, dim3((unsigned)(p.T + kSlotThreads - 1) / kSlotThreads), dim3(kSlotThreads), 0, stream, p);
+    return e;
+}
+
+hipError_t launch_cache_append(const AppendParams& p, int dtype, hipStream_t stream) {
+    const dim3 grid((unsigned)((p.T + p.window - 1) / p.window), (unsigned)(2 * p.H));
+    return launch1(dtype == 0 ? (const void*)cache_append_kernel<_Float16> : (const void*)cache_append_kernel<__bf16>, grid, dim3(256), 0, stream, p);
+}
+
+}  // namespace fa

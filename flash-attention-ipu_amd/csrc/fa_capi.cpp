@@ -12,6 +12,7 @@
 #include <stdio.h>
 #include <string.h>
 
+#include "fa_cache.h"
 #include "fa_extras.h"
 #include "fa_params.h"
 #include "fa_tuning_table.h"
@@ -464,6 +465,11 @@ const OptionName kOptionNames[] = {
 
 }  // namespace
 
+// the same thread-local text for the entry points of fa_cache_capi.cpp
+namespace fa {
+int set_error(int code, const char* text) { return fail(code, "%s", text); }
+}  // namespace fa
+
 extern "C" {
 
 int fa_abi_version(void) { return FA_ABI_VERSION; }
@@ -487,6 +493,7 @@ const char* fa_error_string(int code) {
         case FA_ERR_BAD_OPTION: return "unknown debug option or value out of range";
         case FA_ERR_BAD_MASK: return "bad mask kind or mask pointer";
         case FA_ERR_BAD_DROPOUT: return "dropout_p must be in [0, 1)";
+        case FA_ERR_WORKSPACE: return "workspace too small";
         default: return "unknown error";
     }
 }

@@ -107,6 +107,22 @@ def _declare(lib):
     lib.fa_probe_mfma_peak.argtypes = [i32, i32, i32]
     lib.fa_fwd_qkv_packed.restype = ctypes.c_int
     lib.fa_fwd_qkv_packed.argtypes = [vp, vp, vp, i64, i64, i64, i32, i32, i32, vp]
+    f32 = ctypes.c_float
+    rope = [vp, i64, vp, i32, i64, i64, i64, i64, i64, i64, i64, vp, i32, f32, i32, vp]      # table .. stream
+    lib.fa_qk_norm_rope_fwd.restype = ctypes.c_int
+    lib.fa_qk_norm_rope_fwd.argtypes = [vp] * 6 + [i32] + rope
+    lib.fa_qk_norm_rope_workspace.restype = i64
+    lib.fa_qk_norm_rope_workspace.argtypes = [i64] * 5
+    lib.fa_qk_norm_rope_bwd.restype = ctypes.c_int
+    lib.fa_qk_norm_rope_bwd.argtypes = [vp] * 10 + [i32, vp, i64] + rope
+    lib.fa_cache_tables.restype = ctypes.c_int
+    lib.fa_cache_tables.argtypes = [vp, vp, vp, i64, i64, vp, i64, vp, i64, i64, i64] + [vp] * 7
+    lib.fa_cache_append.restype = ctypes.c_int
+    lib.fa_cache_append.argtypes = [vp] * 7 + [i64] * 6 + [vp, vp, i32, vp]
+    lib.fa_cache_attn_workspace.restype = i64
+    lib.fa_cache_attn_workspace.argtypes = [i64] * 8
+    lib.fa_cache_attn.restype = ctypes.c_int
+    lib.fa_cache_attn.argtypes = [vp] * 10 + [i64] * 12 + [vp, vp, i32, f32, vp]
 
 
 def _raise(rc):

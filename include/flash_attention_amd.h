@@ -76,7 +76,8 @@ enum {
     /* (-13 is unassigned: ABI 4 drafts returned FA_ERR_UNSUPPORTED for a mask / dropout on operands the MFMA kernels do not take; the generic
         kernels have served those since, and the name left the header with ABI 7) */
     FA_ERR_BAD_MASK = -14,          /* mask_kind out of range, or mask pointer and mask_kind disagree */
-    FA_ERR_BAD_DROPOUT = -15        /* dropout_p outside [0, 1) */
+    FA_ERR_BAD_DROPOUT = -15,       /* dropout_p outside [0, 1) */
+    FA_ERR_WORKSPACE = -16          /* workspace missing, misaligned or smaller than the call's *_workspace() says */
 };
 
 /* hardware tile the request was mapped to (fa_plan) */
@@ -273,6 +274,86 @@ int fa_bwd_ex(const void* q, const void* k, const void* v, const void* out, cons
 /* Forward on a contiguous packed qkv [3,G,L,D] -> out [G,L,D] (scale 1, causal). */
 int fa_fwd_qkv_packed(const void* qkv, void* out, float* lse, int64_t G, int64_t L, int64_t D,
                       int32_t num_chunks_q, int32_t num_chunks_kv, int32_t dtype, void* stream);
+
+/* ---- around attention: norm and rotation of queries and keys, and a block cache of 8-bit keys and values --------------------------------
+ * (No reference counterpart: the reference's op takes queries and keys as they are and one whole sequence at a time, sdpa.py:21-41.)
+ * As above: device pointers, caller-owned memory, the caller's stream and current device, no allocation, no synchronisation. */
+
+/*
+ * Norm of every query and key head with the position rotation in one pass:
+ *   y = x / sqrt(mean(x^2) + eps) * weight;  then for the pairs (a, b) of y's first R columns  (a cos - b sin, a sin + b cos).
+ *   q, k, q_out, k_out : element (b, h, l, d) at base + b strides[i][0] + h strides[i][1] + l strides[i][2] + d, i = 0..3 in this order
+ *   q_weight, k_weight : [D] in weight_dtype (the operands' dtype or FA_DTYPE_F32), or NULL for ones
+ *   table     : float32 [table_rows][R]: the cosines of the R / 2 angles of a position, then their sines
+ *   positions : int32 (position_bytes 4) or int64 (8), position of (b, l) at positions[b * position_stride + l]; NULL = l.  A negative position marks a row of
+ *               padding, whose outputs (and gradients) are zeros; a position >= table_rows gives NaN.  The table is never read outside.
+ *   interleaved : 0 = pairs (i, i + R / 2), 1 = pairs (2 i, 2 i + 1)
+ * D even, 2 .. 512; R even, 0 .. D (R = 0: the norm alone, table may be NULL).  D in {32, 64, 128, 256} with R a multiple of 16 and 16-byte rows runs
+ * with 16-byte accesses, everything else one element at a time.  32-bit arithmetic, one rounding at the end.  q_out / k_out may be q / k themselves.
+ */
+int fa_qk_norm_rope_fwd(const void* q, const void* k, void* q_out, void* k_out, const void* q_weight, const void* k_weight, int32_t weight_dtype,
+                        const float* table, int64_t table_rows, const void* positions, int32_t position_bytes, int64_t position_stride, int64_t B, int64_t L,
+                        int64_t heads, int64_t heads_kv, int64_t D, int64_t R, const int64_t strides[4][3], int32_t dtype, float eps, int32_t interleaved,
+                        void* stream);
+/* Its backward: strides of q, k, dq_out, dk_out, dq, dk.  dq_weight / dk_weight: [D] in weight_dtype or NULL; where either is wanted, `workspace` holds
+ * fa_qk_norm_rope_workspace() bytes.  No atomics: results are bit-reproducible from call to call. */
+int64_t fa_qk_norm_rope_workspace(int64_t B, int64_t L, int64_t heads, int64_t heads_kv, int64_t D);
+int fa_qk_norm_rope_bwd(const void* q, const void* k, const void* dq_out, const void* dk_out, void* dq, void* dk, const void* q_weight, const void* k_weight,
+                        void* dq_weight, void* dk_weight, int32_t weight_dtype, void* workspace, int64_t workspace_bytes, const float* table, int64_t table_rows,
+                        const void* positions, int32_t position_bytes, int64_t position_stride, int64_t B, int64_t L, int64_t heads, int64_t heads_kv,
+                        int64_t D, int64_t R, const int64_t strides[6][3], int32_t dtype, float eps, int32_t interleaved, void* stream);
+
+/*
+ * Block tables, positions and slots of one step, from the requests' lengths, all on the device.  Request b holds seq_lens[b] tokens in
+ * ceil(seq_lens[b] / block_size) blocks named by block_tables[b * table_stride + 0 ..]; new_lens[b] tokens come (0 = none, negative = the request ends).
+ * free_blocks[0 .. *free_count - 1] are the free blocks (capacity pool_size).
+ *   - the blocks of the requests that end are put behind the free ones, in the order of the requests and of their blocks;
+ *   - a request is served whole or not at all: its tokens have to end inside num_tokens, its blocks inside max_blocks, and the blocks that all such
+ *     requests up to and including it need have to be free (a request that needs none is served always).  Blocks are taken from the end of the list.
+ *   seq_lens_out [B]  tokens held afterwards (0 for a request that ends); may be seq_lens itself
+ *   free_count_out    may be free_count itself
+ *   cu_new [B + 1]    running sum of max(new_lens, 0);   granted [B]: the tokens that a request was served, new_lens[b] or 0
+ *   positions, slots [num_tokens]  of the tokens in request order; slot = block * block_size + offset.  -1 for tokens that were not served and
+ *                     for the rows behind the last request's.
+ * block_tables is changed only where blocks are added (the entries of a request that ends stay: seq_lens = 0 puts them out of reach).
+ */
+int fa_cache_tables(const int32_t* seq_lens, const int32_t* new_lens, int32_t* block_tables, int64_t table_stride, int64_t max_blocks, int32_t* free_blocks,
+                    int64_t pool_size, const int32_t* free_count, int64_t num_requests, int64_t num_tokens, int64_t block_size, int32_t* seq_lens_out,
+                    int32_t* free_count_out, int32_t* cu_new, int32_t* granted, int32_t* positions, int32_t* slots, void* stream);
+
+/*
+ * New keys and values into a block cache of OCP e4m3 codes with one float32 scale per block and head (value = code * scale):
+ *   k_cache [num_blocks][heads_kv][block_size][W],  v_cache [num_blocks][heads_kv][W][block_size],  k_scale, v_scale [num_blocks][heads_kv]
+ *   W = D rounded up to a multiple of 64 (columns D .. W - 1 are written as zeros); block_size 16, 32, 64 or 128
+ *   block_strides = {bytes between two blocks of k_cache, of v_cache, elements between two blocks' k_scale, v_scale}: a layer's part of a larger
+ *   allocation can be addressed; everything inside a block is contiguous
+ *   k, v : element (t, h, d) at base + t * token_strides[0 | 2] + h * token_strides[1 | 3] + d, f16 or bf16, 16-byte rows
+ *   slots [num_tokens] : where a token goes; negative or not inside the cache = the token is skipped
+ * Tokens whose slots follow each other inside a block form a run (fa_cache_tables lays them so).  A run that starts its block sets the scale to
+ * 2^e, the smallest power of two with max |x| <= 448 * 2^e over the run's finite values (e >= -100); any other run raises the scale to that if it is
+ * larger, and the block's codes are then brought to the new scale.  inf and NaN are stored as NaN.  One call may bring ONE run to a block: with
+ * two runs in the same block, or the same slot twice, that block's contents are unspecified (nothing outside it is touched).
+ */
+int fa_cache_append(const void* k, const void* v, const int32_t* slots, void* k_cache, void* v_cache, float* k_scale, float* v_scale, int64_t num_tokens,
+                    int64_t heads_kv, int64_t D, int64_t W, int64_t num_blocks, int64_t block_size, const int64_t token_strides[4], const int64_t block_strides[4],
+                    int32_t dtype, void* stream);
+
+/*
+ * Causal attention of ragged query runs over that cache.  Request b's queries are the tokens cu_q[b] .. cu_q[b + 1] - 1 of q and out ([num_tokens], heads,
+ * D; token_strides = {token, head stride of q, of out} in elements, 16-byte rows): the LAST of its seq_lens[b] tokens.  Token i of n sees the keys below
+ * seq_lens[b] - n + i + 1; one that sees none (an empty request, a table entry outside the cache) gives zeros.  Query head h reads key/value head
+ * h / (heads / heads_kv).  Rows of out behind cu_q[num_requests] are not written.  Lengths and tables are read on the device only, and held inside the
+ * tensors: no value in them leads to an access outside.  max_q_len: the longest run, as far as the caller knows: it chooses the kernel, and results are
+ * right whatever it is.  The scales have to be >= 0.
+ * workspace: fa_cache_attn_workspace() bytes (negative: an error code), 16-byte aligned, for this call alone while it runs.
+ * Partial sums are joined in a fixed order: results are bit-reproducible from call to call.
+ */
+int64_t fa_cache_attn_workspace(int64_t num_requests, int64_t num_tokens, int64_t heads, int64_t heads_kv, int64_t D, int64_t block_size, int64_t max_blocks,
+                                int64_t max_q_len);
+int fa_cache_attn(const void* q, void* out, const void* k_cache, const void* v_cache, const float* k_scale, const float* v_scale, const int32_t* block_tables,
+                  const int32_t* seq_lens, const int32_t* cu_q, void* workspace, int64_t workspace_bytes, int64_t num_requests, int64_t num_tokens, int64_t heads,
+                  int64_t heads_kv, int64_t D, int64_t W, int64_t num_blocks, int64_t block_size, int64_t max_blocks, int64_t table_stride, int64_t max_q_len,
+                  const int64_t token_strides[4], const int64_t block_strides[4], int32_t dtype, float softmax_scale, void* stream);
 
 #ifdef __cplusplus
 }
