@@ -29,7 +29,9 @@ int64_t up(int64_t a, int64_t b) { return (a + b - 1) / b; }
 bool aligned(const void* p, uintptr_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0; }
 
 // ---- norm and rotation ------------------------------------------------------------------------------------------------------------------
-constexpr int kRopeMaxBlocks = 1024;          // backward: workgroups per side = rows of partial weight gradients
+constexpr int kRopeMaxBlocks = 768;           // backward: workgroups per side = rows of partial weight gradients
+
+constexpr int kRopeFwdBlocks = 2048;          // forward: workgroups per side
 
 struct RopeCall {
     fa::RopeParams p;
@@ -66,6 +68,7 @@ int rope_common(RopeCall* c, const void* q_weight, const void* k_weight, int32_t
     p.L = (int32_t)L; p.D = (int32_t)D; p.R = (int32_t)R; p.interleaved = interleaved; p.w_f32 = weight_dtype == FA_DTYPE_F32; p.eps = eps;
     p.side[0].w = q_weight; p.side[1].w = k_weight;
     p.side[0].heads = (int32_t)heads; p.side[1].heads = (int32_t)heads_kv;
+    if (!aligned(table, 16) || !aligned(q_weight, 16) || !aligned(k_weight, 16)) wide = false;
     c->vec = wide;
     c->es = es;
     return FA_OK;
@@ -83,7 +86,7 @@ void rope_shape(RopeCall* c, int64_t B, bool backward) {
         s.items = (int32_t)(tokens * s.chunks);
         int64_t blocks = up((int64_t)s.items * lpr, 256);
         if (backward && blocks > kRopeMaxBlocks) blocks = kRopeMaxBlocks;
-        if (blocks > (1 << 24)) blocks = 1 << 24;          // (the kernels stride over what is left)
+        if (blocks > kRopeFwdBlocks) blocks = kRopeFwdBlocks;          // (the kernels stride over what is left)
         s.blocks = (int32_t)blocks;
         s.head_inner = s.x_sh <= s.x_sl;
     }
@@ -199,8 +202,8 @@ int fa_qk_norm_rope_bwd(const void* q, const void* k, const void* dq_out, const 
     if (int rc = rope_common(&c, q_weight ? q_weight : dq_weight, k_weight ? k_weight : dk_weight, weight_dtype, table, table_rows, positions, position_bytes,
                              position_stride, B, L, heads, heads_kv, D, R, strides, 6, dtype, eps, interleaved))
         return rc;
-    if ((dq_weight || dk_weight) && (workspace_bytes < fa_qk_norm_rope_workspace(B, L, heads, heads_kv, D) || !aligned(workspace, 4)))
-        return fail(FA_ERR_WORKSPACE, "fa_qk_norm_rope_bwd: workspace must be 4-byte aligned and hold %lld bytes", (long long)fa_qk_norm_rope_workspace(B, L, heads, heads_kv, D));
+    if ((dq_weight || dk_weight) && (workspace_bytes < fa_qk_norm_rope_workspace(B, L, heads, heads_kv, D) || !aligned(workspace, 8)))
+        return fail(FA_ERR_WORKSPACE, "fa_qk_norm_rope_bwd: workspace must be 8-byte aligned and hold %lld bytes", (long long)fa_qk_norm_rope_workspace(B, L, heads, heads_kv, D));
     const void* in[2] = {q, k};
     const void* din[2] = {dq_out, dk_out};
     void* out[2] = {dq, dk};

@@ -60,6 +60,15 @@ __device__ __forceinline__ int64_t row_of(const RopeParams& p, int b, int l) {
     return pos < 0 ? -1 : pos < p.table_rows ? pos : p.table_rows;
 }
 
+// eight weights of columns c .. c + 7 (16-byte aligned; ones without weights)
+template <typename T>
+__device__ __forceinline__ void weights8(const RopeParams& p, const void* w, int c, float (&f)[8]) {
+    if (w == nullptr) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) f[i] = 1.0f;
+    } else if (p.w_f32) load8((const float*)w + c, f);
+    else load8((const T*)w + c, f);
+}
 template <typename T>
 __device__ __forceinline__ float weight_at(const RopeParams& p, const void* w, int i) {
     return w == nullptr ? 1.0f : p.w_f32 ? ((const float*)w)[i] : (float)((const T*)w)[i];
@@ -115,12 +124,10 @@ __global__ __launch_bounds__(256) void rope_vec_kernel(RopeParams p) {
         c1 = R + (D - R) / 2 + 8 * (j - rot);
     }
     float w0[8], w1[8], dw0[8], dw1[8];
+    weights8<T>(p, s.w, c0, w0);
+    weights8<T>(p, s.w, c1, w1);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        w0[i] = weight_at<T>(p, s.w, c0 + i);
-        w1[i] = weight_at<T>(p, s.w, c1 + i);
-        dw0[i] = dw1[i] = 0.f;
-    }
+    for (int i = 0; i < 8; ++i) dw0[i] = dw1[i] = 0.f;
     const T* x = (const T*)s.x;
     const T* dy = (const T*)s.dy;
     T* y = (T*)s.y;
@@ -148,8 +155,8 @@ __global__ __launch_bounds__(256) void rope_vec_kernel(RopeParams p) {
         const bool pad = pos < 0;
         if (rotated && pos >= 0 && pos < p.table_rows) {
             const float* t = p.table + pos * R + 8 * j;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) { cs[i] = t[i]; sn[i] = t[R / 2 + i]; }
+            load8(t, cs);
+            load8(t + R / 2, sn);
         }
         if (pos == p.table_rows) {
 #pragma unroll
@@ -305,24 +312,36 @@ __global__ __launch_bounds__(256) void rope_any_kernel(RopeParams p) {
     }
 }
 
-// dw = sum of the workgroups' rows, in order: 16 columns x 16 row strands per workgroup
+// dw = sum of the workgroups' rows in a fixed order: 64 columns per workgroup, 32 strands of rows, whose loads are independent and in flight together (the
+// kernel is a few microseconds of latency)
+constexpr int kDwStrands = 32;
 template <typename T>
-__global__ __launch_bounds__(256) void rope_dw_kernel(RopeParams p) {
+__global__ __launch_bounds__(1024) void rope_dw_kernel(RopeParams p) {
+    typedef float f32x2 __attribute__((ext_vector_type(2)));
     const RopeSide& s = p.side[blockIdx.y];
     if (s.dw == nullptr) return;
-    const int col = (int)blockIdx.x * 16 + ((int)threadIdx.x & 15), strand = (int)threadIdx.x >> 4;
-    __shared__ float part[16][17];
-    float sum = 0.f;
-    if (col < p.D)
-        for (int r = strand; r < s.blocks; r += 16) sum += s.dw_part[(int64_t)r * p.D + col];
-    part[strand][threadIdx.x & 15] = sum;
+    const int tid = (int)threadIdx.x, c = tid & 31, strand = tid >> 5, col = (int)blockIdx.x * 64 + 2 * c;
+    __shared__ f32x2 part[16][32];
+    f32x2 sum = {0.f, 0.f};
+    if (col < p.D) {
+#pragma unroll 8
+        for (int r = strand; r < s.blocks; r += kDwStrands) sum += *(const f32x2*)(s.dw_part + (int64_t)r * p.D + col);
+    }
+    sum[0] += __shfl_xor(sum[0], 32);
+    sum[1] += __shfl_xor(sum[1], 32);
+    if ((strand & 1) == 0) part[strand >> 1][c] = sum;
     __syncthreads();
-    if (strand == 0 && col < p.D) {
-        sum = 0.f;
+    if (tid < 32 && col < p.D) {
+        sum = part[0][c];
 #pragma unroll
-        for (int r = 0; r < 16; ++r) sum += part[r][threadIdx.x & 15];
-        if (p.w_f32) ((float*)s.dw)[col] = sum;
-        else ((T*)s.dw)[col] = (T)sum;
+        for (int r = 1; r < 16; ++r) sum += part[r][c];
+        if (p.w_f32) {
+            ((float*)s.dw)[col] = sum[0];
+            ((float*)s.dw)[col + 1] = sum[1];
+        } else {
+            ((T*)s.dw)[col] = (T)sum[0];
+            ((T*)s.dw)[col + 1] = (T)sum[1];
+        }
     }
 }
 
@@ -342,7 +361,7 @@ hipError_t launch_rope(const RopeParams& p, bool vec, int hc, hipStream_t stream
     const void* k = !vec ? (const void*)rope_any_kernel<T, BWD> : p.interleaved ? vec_kernel<T, true, BWD>(p.D, hc) : vec_kernel<T, false, BWD>(p.D, hc);
     hipError_t e = launch1(k, grid, dim3(256), 0, stream, p);
     if (e == hipSuccess && BWD && (p.side[0].dw || p.side[1].dw))
-        e = launch1((const void*)rope_dw_kernel<T>, dim3((unsigned)(p.D + 15) / 16, 2), dim3(256), 0, stream, p);
+        e = launch1((const void*)rope_dw_kernel<T>, dim3((unsigned)(p.D + 63) / 64, 2), dim3(1024), 0, stream, p);
     return e;
 }
 

@@ -318,6 +318,19 @@ def _stream_for(t: torch.Tensor):
     return (_raw_stream(cur) if _raw_stream is not None else torch.cuda.current_stream(cur).cuda_stream), prev
 
 
+_get_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+
+
+def stream_of(device: torch.device):
+    """(raw stream of a device that holds tensors, device to go back to or -1): _stream_for without torch.cuda's initialisation checks"""
+    idx, cur = device.index, _get_device()
+    prev = -1
+    if cur != idx:
+        prev = cur
+        torch.cuda.set_device(idx)
+    return (_raw_stream(idx) if _raw_stream is not None else torch.cuda.current_stream(idx).cuda_stream), prev
+
+
 def fwd_bhld(q, k, v, out, lse_ptr, num_chunks_q, num_chunks_kv, scale, causal):
     """fa_fwd on [B, H, L, D] views (k / v may carry fewer heads) with unit stride on D; lse_ptr: device address of [B * H, L] fp32 or None."""
     lib = _LIB or load_native_library()

@@ -25,6 +25,16 @@ def _i64x4(key):
     return blk
 
 
+_LAYOUTS = {}       # (shapes, strides, dtypes) that passed the checks -> what the call needs of them
+
+
+def _remember(key, value):
+    if len(_LAYOUTS) > 4096:
+        _LAYOUTS.clear()
+    _LAYOUTS[key] = value
+    return value
+
+
 def cache_width(head_dim: int) -> int:
     """columns that a head takes in the cache: the head dim rounded up to a multiple of 64"""
     return (head_dim + 63) // 64 * 64
@@ -59,16 +69,10 @@ def _table(name, block_tables, requests):
     return block_tables.shape[1], block_tables.stride(0) if requests > 1 else block_tables.shape[1]
 
 
-def _one_device(name, first, *others):
-    for t in others:
-        if t.device != first.device:
-            raise ValueError(f"{name}: all tensors must be on one device")
-
-
 def _tables_call(seq_lens, new_lens, block_tables, free_blocks, free_count, num_tokens, block_size, seq_out, free_out, cu_new, granted, positions, slots):
     lib = _native._LIB or _native.load_native_library()
     B = seq_lens.shape[0]
-    stream, prev = _native._stream_for(seq_lens)
+    stream, prev = _native.stream_of(seq_lens.device)
     try:
         rc = lib.fa_cache_tables(seq_lens.data_ptr(), new_lens.data_ptr(), block_tables.data_ptr(), block_tables.stride(0) if B > 1 else block_tables.shape[1],
                                  block_tables.shape[1], free_blocks.data_ptr(), free_blocks.shape[0], free_count.data_ptr(), B, num_tokens, block_size,
@@ -87,6 +91,27 @@ def _tables_op(seq_lens: torch.Tensor, new_lens: torch.Tensor, block_tables: tor
     _tables_call(seq_lens, new_lens, block_tables, free_blocks, free_count, num_tokens, block_size, seq_out, free_out, cu_new, granted, positions, slots)
 
 
+def _check_tables(seq_lens, new_lens, block_tables, free_blocks, free_count, num_tokens, block_size, inplace):
+    """(int32 values of the outputs in all, one by one)"""
+    name = "cache_tables"
+    if seq_lens.ndim != 1 or seq_lens.shape[0] < 1:
+        raise ValueError(f"{name}: seq_lens must be [requests] (got {tuple(seq_lens.shape)})")
+    B = seq_lens.shape[0]
+    _ints(name, "seq_lens", seq_lens)
+    _ints(name, "new_lens", new_lens, (B,))
+    _ints(name, "free_count", free_count, (1,))
+    _ints(name, "free_blocks", free_blocks)
+    if free_blocks.ndim != 1 or free_blocks.shape[0] < 1:
+        raise ValueError(f"{name}: free_blocks must be [blocks] (got {tuple(free_blocks.shape)})")
+    _table(name, block_tables, B)
+    if block_size not in BLOCK_SIZES:
+        raise ValueError(f"{name}: block_size must be one of {BLOCK_SIZES} (got {block_size})")
+    if num_tokens < 0:
+        raise ValueError(f"{name}: num_tokens must be >= 0 (got {num_tokens})")
+    sizes = [B + 1, B, num_tokens, num_tokens] + ([] if inplace else [B, 1])
+    return sum(sizes), sizes
+
+
 def cache_tables(seq_lens: torch.Tensor, new_lens: torch.Tensor, block_tables: torch.Tensor, free_blocks: torch.Tensor, free_count: torch.Tensor, num_tokens: int,
                  block_size: int, inplace: bool = False) -> CacheStep:
     """
@@ -102,26 +127,18 @@ def cache_tables(seq_lens: torch.Tensor, new_lens: torch.Tensor, block_tables: t
     A request is served whole or not at all (granted): its tokens have to end inside num_tokens, its blocks have to fit its table row, and the pool has
     to hold what all such requests up to and including it need.  Nothing is read back: look at `granted` when the host next waits for the device.
     """
-    name = "cache_tables"
-    if seq_lens.ndim != 1 or seq_lens.shape[0] < 1:
-        raise ValueError(f"{name}: seq_lens must be [requests] (got {tuple(seq_lens.shape)})")
-    B, dev = seq_lens.shape[0], seq_lens.device
-    _ints(name, "seq_lens", seq_lens)
-    _ints(name, "new_lens", new_lens, (B,))
-    _ints(name, "free_count", free_count, (1,))
-    _ints(name, "free_blocks", free_blocks)
-    if free_blocks.ndim != 1 or free_blocks.shape[0] < 1:
-        raise ValueError(f"{name}: free_blocks must be [blocks] (got {tuple(free_blocks.shape)})")
-    _table(name, block_tables, B)
-    _one_device(name, seq_lens, new_lens, block_tables, free_blocks, free_count)
-    if block_size not in BLOCK_SIZES:
-        raise ValueError(f"{name}: block_size must be one of {BLOCK_SIZES} (got {block_size})")
-    if num_tokens < 0:
-        raise ValueError(f"{name}: num_tokens must be >= 0 (got {num_tokens})")
+    key = (seq_lens.shape, seq_lens.stride(), seq_lens.dtype, new_lens.shape, new_lens.stride(), new_lens.dtype, block_tables.shape, block_tables.stride(), block_tables.dtype,
+           free_blocks.shape, free_blocks.stride(), free_blocks.dtype, free_count.shape, free_count.dtype, num_tokens, block_size, inplace)
+    sizes = _LAYOUTS.get(key)
+    dev = seq_lens.device
+    if sizes is None:
+        sizes = _remember(key, _check_tables(seq_lens, new_lens, block_tables, free_blocks, free_count, num_tokens, block_size, inplace))
+    if not (seq_lens.is_cuda and new_lens.device == dev and block_tables.device == dev and free_blocks.device == dev and free_count.device == dev):
+        raise ValueError("cache_tables: all tensors must be on one GPU")
     # one allocation: cu_new, granted, positions, slots and, unless in place, lengths and count
-    sizes = [B + 1, B, num_tokens, num_tokens] + ([] if inplace else [B, 1])
-    cu_new, granted, positions, slots, *rest = torch.empty(sum(sizes), dtype=torch.int32, device=dev).split(sizes)
-    seq_out, free_out = (seq_lens, free_count) if inplace else rest
+    parts = torch.split_with_sizes(torch.empty(sizes[0], dtype=torch.int32, device=dev), sizes[1])
+    cu_new, granted, positions, slots = parts[:4]
+    seq_out, free_out = (seq_lens, free_count) if inplace else parts[4:]
     call = _tables_op if torch.compiler.is_compiling() else _tables_call
     call(seq_lens, new_lens, block_tables, free_blocks, free_count, num_tokens, block_size, seq_out, free_out, cu_new, granted, positions, slots)
     return CacheStep(seq_out, free_out, cu_new, granted, positions, slots)
@@ -153,16 +170,6 @@ def _check_cache(name, k_cache, v_cache, k_scale, v_scale, heads_kv, D):
     return W, N, P, (ks[0], vs[0], kss, vss)
 
 
-_LAYOUTS = {}       # (shapes, strides, dtypes) that passed the checks -> what the call needs of them
-
-
-def _remember(key, value):
-    if len(_LAYOUTS) > 4096:
-        _LAYOUTS.clear()
-    _LAYOUTS[key] = value
-    return value
-
-
 def _append_call(k, v, slots, k_cache, v_cache, k_scale, v_scale):
     name = "cache_append"
     key = (k.shape, k.stride(), v.shape, v.stride(), k.dtype, v.dtype, slots.shape, slots.dtype, k_cache.shape, k_cache.stride(), v_cache.shape, v_cache.stride(),
@@ -190,7 +197,7 @@ def _append_call(k, v, slots, k_cache, v_cache, k_scale, v_scale):
     T, H, D = k.shape
     if T == 0:
         return
-    stream, prev = _native._stream_for(k)
+    stream, prev = _native.stream_of(dev)
     try:
         rc = lib.fa_cache_append(kp, vp, slots.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), T, H, D, W, N, P, tokens,
                                  strides, dtype, stream)
@@ -273,7 +280,7 @@ def _attn_call(q, k_cache, v_cache, k_scale, v_scale, block_tables, seq_lens, cu
         tokens = _i64x4((q.stride(0), q.stride(1), out.stride(0), out.stride(1)))
     # (a workspace of its own for every call: the allocator orders its reuse on the stream, and a captured graph keeps the one it was captured with)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-    stream, prev = _native._stream_for(q)
+    stream, prev = _native.stream_of(dev)
     try:
         rc = lib.fa_cache_attn(q.data_ptr(), out.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), block_tables.data_ptr(),
                                seq_lens.data_ptr(), cu_q.data_ptr(), ws.data_ptr(), nbytes, *sizes, tokens, strides, dtype, softmax_scale, stream)

@@ -30,64 +30,62 @@ def _strides(t):
     return (st[0], st[1], st[2]) if len(st) == 4 else (0, st[1], st[0])
 
 
-def _like(t: torch.Tensor) -> torch.Tensor:
-    """uninitialised, in t's layout: heads inside the rows if t has them there, contiguous otherwise"""
-    if t.ndim == 4 and t.stride(1) < t.stride(2):
-        B, H, L, D = t.shape
-        return t.new_empty_strided((B, H, L, D), (L * H * D, D, H * D, 1))
-    return t.new_empty(t.shape)
-
-
 _I64x12, _I64x18 = ctypes.c_int64 * 12, ctypes.c_int64 * 18
-_BLOCKS = {}
+_CALLS = {}         # layout of the operands -> what the native calls need of it
 
 
-def _stride_args(tensors):
-    key = tuple(t.stride() for t in tensors)
-    blk = _BLOCKS.get(key)
-    if blk is None:
-        if len(_BLOCKS) > 4096:
-            _BLOCKS.clear()
-        flat = [x for t in tensors for x in _strides(t)]
-        blk = _BLOCKS[key] = (_I64x12 if len(tensors) == 4 else _I64x18)(*flat)
-    return blk
+class _Call:
+    """Everything about a call that follows from shapes, strides and dtypes: checked and formed once for each of them."""
+
+    __slots__ = ("sizes", "table_rows", "position_bytes", "position_stride", "weight_dtype", "dtype", "fwd_strides", "bwd_strides", "workspace")
+
+    def __init__(self, q, k, q_weight, k_weight, table, positions):
+        if q.ndim == 4:
+            B, H, L, D = q.shape
+        else:
+            L, H, D = q.shape
+            B = 1
+        self.sizes = (B, L, H, k.shape[1], D, table.shape[1])
+        self.table_rows = table.shape[0]
+        self.position_bytes = 4 if positions is None else positions.element_size()
+        self.position_stride = positions.stride(0) if positions is not None and positions.ndim == 2 else 0
+        weight = q_weight if q_weight is not None else k_weight
+        self.dtype = _native.FA_DTYPE[q.dtype]
+        self.weight_dtype = self.dtype if weight is None else _native.FA_DTYPE[weight.dtype]
+        self.fwd_strides = None
+        self.bwd_strides = {}
+        self.workspace = _native.load_native_library().fa_qk_norm_rope_workspace(B, L, H, k.shape[1], D)
 
 
-def _geometry(q, k, table, positions):
-    """(table pointer, rows, positions pointer, their bytes, their batch stride, B, L, heads, heads_kv, D, R)"""
-    if q.ndim == 4:
-        B, H, L, D = q.shape
-    else:
-        L, H, D = q.shape
-        B = 1
-    rows, R = table.shape
-    if positions is None:
-        ptr, nbytes, pos_sb = None, 4, 0
-    else:
-        ptr, nbytes = positions.data_ptr(), positions.element_size()
-        pos_sb = positions.stride(0) if positions.ndim == 2 else 0
-    return table.data_ptr(), rows, ptr, nbytes, pos_sb, B, L, H, k.shape[1], D, R
-
-
-def _weight_dtype(q, w):
-    return _native.FA_DTYPE[q.dtype if w is None else w.dtype]
-
-
-def _ptr(t):
-    return None if t is None else t.data_ptr()
+def _call_for(q, k, q_weight, k_weight, table, positions):
+    key = (q.shape, q.stride(), q.dtype, k.shape, k.stride(), k.dtype, None if q_weight is None else (q_weight.shape, q_weight.stride(), q_weight.dtype),
+           None if k_weight is None else (k_weight.shape, k_weight.stride(), k_weight.dtype), table.shape, table.stride(), table.dtype,
+           None if positions is None else (positions.shape, positions.stride(), positions.dtype))
+    call = _CALLS.get(key)
+    if call is None:
+        _check(q, k, q_weight, k_weight, table, positions)
+        if len(_CALLS) > 4096:
+            _CALLS.clear()
+        call = _CALLS[key] = _Call(q, k, q_weight, k_weight, table, positions)
+    dev = q.device
+    if not (q.is_cuda and k.device == dev and table.device == dev and (q_weight is None or q_weight.device == dev) and (k_weight is None or k_weight.device == dev)
+            and (positions is None or positions.device == dev)):
+        raise ValueError("qk_norm_rope: all tensors must be on one GPU")
+    return call
 
 
 def _fwd_impl(q, k, q_weight, k_weight, table, positions, eps, interleaved):
-    q, k = (t if t.stride(-1) == 1 else t.contiguous() for t in (q, k))
-    q_out, k_out = _like(q), _like(k)
-    if q.numel() and k.numel():
-        lib = _native.load_native_library()
-        geo = _geometry(q, k, table, positions)
-        stream, prev = _native._stream_for(q)
+    call = _call_for(q, k, q_weight, k_weight, table, positions)
+    q_out, k_out = torch.empty_like(q), torch.empty_like(k)          # (the operands' layout: heads inside the rows stay there)
+    if call.sizes[0] and call.sizes[1]:
+        if call.fwd_strides is None:
+            call.fwd_strides = _I64x12(*(x for t in (q, k, q_out, k_out) for x in _strides(t)))
+        stream, prev = _native.stream_of(q.device)
         try:
-            rc = lib.fa_qk_norm_rope_fwd(q.data_ptr(), k.data_ptr(), q_out.data_ptr(), k_out.data_ptr(), _ptr(q_weight), _ptr(k_weight),
-                                         _weight_dtype(q, q_weight if q_weight is not None else k_weight), *geo, _stride_args((q, k, q_out, k_out)),
-                                         _native.FA_DTYPE[q.dtype], eps, 1 if interleaved else 0, stream)
+            rc = _native._LIB.fa_qk_norm_rope_fwd(q.data_ptr(), k.data_ptr(), q_out.data_ptr(), k_out.data_ptr(), None if q_weight is None else q_weight.data_ptr(),
+                                                  None if k_weight is None else k_weight.data_ptr(), call.weight_dtype, table.data_ptr(), call.table_rows,
+                                                  None if positions is None else positions.data_ptr(), call.position_bytes, call.position_stride, *call.sizes,
+                                                  call.fwd_strides, call.dtype, eps, interleaved, stream)
         finally:
             if prev >= 0:
                 torch.cuda.set_device(prev)
@@ -97,29 +95,37 @@ def _fwd_impl(q, k, q_weight, k_weight, table, positions, eps, interleaved):
 
 
 def _bwd_impl(q, k, dq_out, dk_out, q_weight, k_weight, table, positions, eps, interleaved, need_q_weight, need_k_weight):
-    q, k, dq_out, dk_out = (t if t.stride(-1) == 1 else t.contiguous() for t in (q, k, dq_out, dk_out))
-    dq, dk = _like(q), _like(k)
+    call = _call_for(q, k, q_weight, k_weight, table, positions)
+    if dq_out.stride(-1) != 1 or dk_out.stride(-1) != 1:
+        dq_out, dk_out = dq_out.contiguous(), dk_out.contiguous()
+    dq, dk = torch.empty_like(q), torch.empty_like(k)
     dqw = torch.empty_like(q_weight) if need_q_weight else None
     dkw = torch.empty_like(k_weight) if need_k_weight else None
-    if q.numel() and k.numel():
-        lib = _native.load_native_library()
-        geo = _geometry(q, k, table, positions)
-        ws, nbytes = None, 0
-        if need_q_weight or need_k_weight:
-            nbytes = lib.fa_qk_norm_rope_workspace(*geo[5:10])
-            ws = torch.empty(nbytes // 4, dtype=torch.float32, device=q.device)
-        stream, prev = _native._stream_for(q)
-        try:
-            rc = lib.fa_qk_norm_rope_bwd(q.data_ptr(), k.data_ptr(), dq_out.data_ptr(), dk_out.data_ptr(), dq.data_ptr(), dk.data_ptr(), _ptr(q_weight), _ptr(k_weight),
-                                         _ptr(dqw), _ptr(dkw), _weight_dtype(q, q_weight if q_weight is not None else k_weight), _ptr(ws), nbytes, *geo,
-                                         _stride_args((q, k, dq_out, dk_out, dq, dk)), _native.FA_DTYPE[q.dtype], eps, 1 if interleaved else 0, stream)
-        finally:
-            if prev >= 0:
-                torch.cuda.set_device(prev)
-        if rc != 0:
-            _native._raise(rc)
-    else:
-        dqw, dkw = (None if w is None else w.zero_() for w in (dqw, dkw))
+    if not (call.sizes[0] and call.sizes[1]):
+        return dq, dk, None if dqw is None else dqw.zero_(), None if dkw is None else dkw.zero_()
+    key = (dq_out.stride(), dk_out.stride())
+    strides = call.bwd_strides.get(key)
+    if strides is None:
+        if len(call.bwd_strides) > 256:
+            call.bwd_strides.clear()
+        strides = call.bwd_strides[key] = _I64x18(*(x for t in (q, k, dq_out, dk_out, dq, dk) for x in _strides(t)))
+    ws, nbytes = None, 0
+    if need_q_weight or need_k_weight:
+        nbytes = call.workspace
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
+    stream, prev = _native.stream_of(q.device)
+    try:
+        rc = _native._LIB.fa_qk_norm_rope_bwd(q.data_ptr(), k.data_ptr(), dq_out.data_ptr(), dk_out.data_ptr(), dq.data_ptr(), dk.data_ptr(),
+                                              None if q_weight is None else q_weight.data_ptr(), None if k_weight is None else k_weight.data_ptr(),
+                                              None if dqw is None else dqw.data_ptr(), None if dkw is None else dkw.data_ptr(), call.weight_dtype,
+                                              None if ws is None else ws.data_ptr(), nbytes, table.data_ptr(), call.table_rows,
+                                              None if positions is None else positions.data_ptr(), call.position_bytes, call.position_stride, *call.sizes, strides,
+                                              call.dtype, eps, interleaved, stream)
+    finally:
+        if prev >= 0:
+            torch.cuda.set_device(prev)
+    if rc != 0:
+        _native._raise(rc)
     return dq, dk, dqw, dkw
 
 
@@ -132,8 +138,7 @@ def _op(q: torch.Tensor, k: torch.Tensor, q_weight: Optional[torch.Tensor], k_we
 
 @_op.register_fake
 def _(q, k, q_weight, k_weight, table, positions, eps, interleaved):
-    q, k = (t if t.stride(-1) == 1 else t.contiguous() for t in (q, k))
-    return _like(q), _like(k)
+    return torch.empty_like(q), torch.empty_like(k)
 
 
 @custom_op("flash_attention_amd::qk_norm_rope_bwd", mutates_args=())
@@ -146,8 +151,7 @@ def _op_bwd(q: torch.Tensor, k: torch.Tensor, dq_out: torch.Tensor, dk_out: torc
 
 @_op_bwd.register_fake
 def _(q, k, dq_out, dk_out, q_weight, k_weight, table, positions, eps, interleaved):
-    q, k = (t if t.stride(-1) == 1 else t.contiguous() for t in (q, k))
-    return (_like(q), _like(k), q.new_empty(0) if q_weight is None else torch.empty_like(q_weight),
+    return (torch.empty_like(q), torch.empty_like(k), q.new_empty(0) if q_weight is None else torch.empty_like(q_weight),
             q.new_empty(0) if k_weight is None else torch.empty_like(k_weight))
 
 
@@ -166,6 +170,15 @@ def _op_backward(ctx, dq_out, dk_out):
 _op.register_autograd(_op_backward, setup_context=_op_setup)
 
 
+def _backward(ctx, dq_out, dk_out):
+    q, k, q_weight, k_weight, table, positions = ctx.saved_tensors
+    need = ctx.needs_input_grad
+    return (*_bwd_impl(q, k, dq_out, dk_out, q_weight, k_weight, table, positions, ctx.eps, ctx.interleaved, need[2], need[3]), None, None, None, None)
+
+
+_backward_once = once_differentiable(_backward)
+
+
 class _QkNormRopeFn(torch.autograd.Function):
     """eager path: the same two calls without the dispatcher's cost"""
 
@@ -176,17 +189,14 @@ class _QkNormRopeFn(torch.autograd.Function):
         return _fwd_impl(q, k, q_weight, k_weight, table, positions, eps, interleaved)
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dq_out, dk_out):
-        q, k, q_weight, k_weight, table, positions = ctx.saved_tensors
-        need = ctx.needs_input_grad
-        dq, dk, dqw, dkw = _bwd_impl(q, k, dq_out, dk_out, q_weight, k_weight, table, positions, ctx.eps, ctx.interleaved, need[2], need[3])
-        return dq, dk, dqw, dkw, None, None, None, None
+        # (a double backward raises; the wrapper that sees to it costs 10 us a call and matters only where a graph of the backward is asked for)
+        if torch.is_grad_enabled():
+            return _backward_once(ctx, dq_out, dk_out)
+        return _backward(ctx, dq_out, dk_out)
 
 
-
-
-def _check(q, k, q_weight, k_weight, table, positions, eps):
+def _check(q, k, q_weight, k_weight, table, positions):
     name = "qk_norm_rope"
     if not (q.is_cuda and k.is_cuda and table.is_cuda):
         raise ValueError(f"{name} needs GPU tensors")
@@ -211,12 +221,6 @@ def _check(q, k, q_weight, k_weight, table, positions, eps):
             raise TypeError(f"{name}: positions must be int32 or int64 (got {positions.dtype})")
         if tuple(positions.shape) not in ((tokens, tokens[1:]) if len(tokens) == 2 else (tokens,)):
             raise ValueError(f"{name}: positions must be [L] or [B, L] for [B, H, L, D], [T] for [T, H, D] (got {tuple(positions.shape)})")
-    if any(t.device != q.device for t in (k, table, *weights, *(() if positions is None else (positions,)))):
-        raise ValueError(f"{name}: all tensors must be on one device")
-    if table.requires_grad:
-        raise ValueError(f"{name} has no gradient for the table")
-    if not 0.0 <= eps < float("inf"):
-        raise ValueError(f"{name}: eps must be finite and >= 0 (got {eps})")
 
 
 def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: Optional[torch.Tensor], k_weight: Optional[torch.Tensor], table: torch.Tensor,
@@ -232,12 +236,18 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: Optional[torch.Tens
     interleaved False: columns (i, i + rotary dim / 2) are a pair; True: (2 i, 2 i + 1)
     returns     (q, k) normed and rotated, in the operands' layout
     """
-    _check(q, k, q_weight, k_weight, table, positions, eps)
-    if positions is not None and positions.ndim and positions.stride(-1) != 1 and positions.shape[-1] > 1:
+    if not 0.0 <= eps < float("inf"):
+        raise ValueError(f"qk_norm_rope: eps must be finite and >= 0 (got {eps})")
+    if q.stride(-1) != 1 or k.stride(-1) != 1:
+        q, k = q.contiguous(), k.contiguous()
+    if positions is not None and positions.ndim and positions.stride(-1) != 1:
         positions = positions.contiguous()
     if torch.compiler.is_compiling():
+        _check(q, k, q_weight, k_weight, table, positions)
         return _op(q, k, q_weight, k_weight, table, positions, float(eps), bool(interleaved))
-    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or (q_weight is not None and q_weight.requires_grad)
-                                    or (k_weight is not None and k_weight.requires_grad)):
-        return _QkNormRopeFn.apply(q, k, q_weight, k_weight, table, positions, float(eps), bool(interleaved))
-    return _fwd_impl(q, k, q_weight, k_weight, table, positions, float(eps), bool(interleaved))
+    if torch.is_grad_enabled():
+        if table.requires_grad:
+            raise ValueError("qk_norm_rope has no gradient for the table")
+        if q.requires_grad or k.requires_grad or (q_weight is not None and q_weight.requires_grad) or (k_weight is not None and k_weight.requires_grad):
+            return _QkNormRopeFn.apply(q, k, q_weight, k_weight, table, positions, eps, interleaved)
+    return _fwd_impl(q, k, q_weight, k_weight, table, positions, eps, interleaved)
