@@ -177,19 +177,36 @@ __global__ __launch_bounds__(kSlotThreads) void cache_slots_kernel(TablesParams 
 // several short ones by a wave each.
 // A work item is eight columns of four consecutive tokens: 16-byte loads, the values stay in registers between the maximum and the codes, and
 // both layouts store whole words - eight bytes of a key row, or (columns down the lanes) four tokens of a value column.
-template <typename T> struct Bits;
-template <> struct Bits<_Float16> {
-    static constexpr unsigned top = 0x7c00u;
-    static __device__ __forceinline__ float f(unsigned u) { return (float)__builtin_bit_cast(_Float16, (unsigned short)u); }
-};
-template <> struct Bits<__bf16> {
-    static constexpr unsigned top = 0x7f80u;
-    static __device__ __forceinline__ float f(unsigned u) { return __builtin_bit_cast(float, u << 16); }
-};
-
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
 typedef unsigned u32x4v __attribute__((ext_vector_type(4)));
+typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+typedef short s16x2 __attribute__((ext_vector_type(2)));
+
+template <typename T> struct Bits;
+template <> struct Bits<_Float16> {
+    static constexpr unsigned top = 0x7c00u;
+    typedef _Float16 vec2 __attribute__((ext_vector_type(2)));
+    static __device__ __forceinline__ float f(unsigned u) { return (float)__builtin_bit_cast(_Float16, (unsigned short)u); }
+    // four finite values / 2^e -> four codes, one rounding: the instruction divides by the scale's power of two before it rounds
+    static __device__ __forceinline__ unsigned codes(unsigned a, unsigned b, float scale) {
+        s16x2 r = {0, 0};
+        r = __builtin_amdgcn_cvt_scalef32_pk_fp8_f16(r, __builtin_bit_cast(vec2, a), scale, false);
+        r = __builtin_amdgcn_cvt_scalef32_pk_fp8_f16(r, __builtin_bit_cast(vec2, b), scale, true);
+        return __builtin_bit_cast(unsigned, r);
+    }
+};
+template <> struct Bits<__bf16> {
+    static constexpr unsigned top = 0x7f80u;
+    typedef __bf16 vec2 __attribute__((ext_vector_type(2)));
+    static __device__ __forceinline__ float f(unsigned u) { return __builtin_bit_cast(float, u << 16); }
+    static __device__ __forceinline__ unsigned codes(unsigned a, unsigned b, float scale) {
+        s16x2 r = {0, 0};
+        r = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(r, __builtin_bit_cast(vec2, a), scale, false);
+        r = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(r, __builtin_bit_cast(vec2, b), scale, true);
+        return __builtin_bit_cast(unsigned, r);
+    }
+};
 
 // |x| <= 448 by the choice of the scale, except inf and NaN, which become the code of NaN
 __device__ __forceinline__ unsigned codes2(float a, float b) {
@@ -216,58 +233,91 @@ __device__ __forceinline__ unsigned wave_max(unsigned x) {
     }
     return x;
 }
+// bytes of four rows of four -> four columns of four
+__device__ __forceinline__ void transpose4(unsigned (&r)[4]) {
+    const unsigned a = __builtin_amdgcn_perm(r[1], r[0], 0x05010400u), b = __builtin_amdgcn_perm(r[1], r[0], 0x07030602u);
+    const unsigned c = __builtin_amdgcn_perm(r[3], r[2], 0x05010400u), d = __builtin_amdgcn_perm(r[3], r[2], 0x07030602u);
+    r[0] = __builtin_amdgcn_perm(c, a, 0x05040100u);
+    r[1] = __builtin_amdgcn_perm(c, a, 0x07060302u);
+    r[2] = __builtin_amdgcn_perm(d, b, 0x05040100u);
+    r[3] = __builtin_amdgcn_perm(d, b, 0x07060302u);
+}
 
 // one run: tokens t0 .. t0 + n - 1 into positions off .. off + n - 1 of a block.  NT = 64 (a wave) or 256 (the workgroup)
-template <typename T, bool KEYS, int NT>
+template <typename T, int W, bool KEYS, int NT>
 __device__ __forceinline__ void append_run(const AppendParams& p, int t0, int n, int64_t block, int off, int head, unsigned* shared_max) {
+    constexpr int S = KEYS ? 0 : 1, WC = W / 8;                           // column chunks of a row
     const int tid = (int)threadIdx.x & (NT - 1);
-    const int P = 1 << p.shift, W = p.W, chunks = p.D >> 3, wchunks = W >> 3;
+    const int P = 1 << p.shift, chunks = p.D >> 3;
     const int g0 = off >> 2, groups = ((off + n + 3) >> 2) - g0;          // groups of four positions that the run touches
-    const T* x = (const T*)p.x[KEYS ? 0 : 1] + (int64_t)head * p.x_sh[KEYS ? 0 : 1];
-    const int64_t st = p.x_st[KEYS ? 0 : 1];
-    uint8_t* tile = (uint8_t*)p.cache[KEYS ? 0 : 1] + block * p.block_stride[KEYS ? 0 : 1] + (int64_t)head * P * W;
-    float* scale = p.scale[KEYS ? 0 : 1] + block * p.scale_stride[KEYS ? 0 : 1] + head;
+    // keys: neighbouring lanes take a row's chunks; values: neighbouring lanes take up to sixteen groups of one chunk (a 64-byte piece of every column)
+    const int lg = groups > 4 ? 4 : groups > 1 ? 2 : 0;
+    const int items = KEYS ? groups * WC : (((groups - 1) >> lg) + 1) * (WC << lg);
+    const int64_t st = p.x_st[S];
+    const T* x = (const T*)p.x[S] + (int64_t)head * p.x_sh[S] + (int64_t)t0 * st;
+    uint8_t* tile = (uint8_t*)p.cache[S] + block * p.block_stride[S] + (int64_t)head * P * W;
+    float* scale = p.scale[S] + block * p.scale_stride[S] + head;
     const float old = off ? *scale : 0.f;
 
-    const auto load = [&](int i, u32x4v (&v)[4], int& g, int& c) {        // item i: position group g, column chunk c
-        if (KEYS) { g = g0 + i / wchunks; c = i % wchunks; }
-        else { g = g0 + i % groups; c = i / groups; }
+    const auto place = [&](int i, int& g, int& c) {                       // item i: position group g, column chunk c
+        if (KEYS) { g = g0 + i / WC; c = i % WC; }
+        else { const int hi = i >> lg; g = g0 + ((hi / WC) << lg) + (i & ((1 << lg) - 1)); c = hi % WC; }
+    };
+    const auto load = [&](int i, u32x4v (&v)[4]) {
+        int g, c;
+        place(i, g, c);
+        const int k0 = 4 * g - off;                                       // run index of the group's first position
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-            const int k = 4 * g + r - off;
-            if (k >= 0 && k < n && c < chunks) v[r] = *(const u32x4v*)(x + (int64_t)(t0 + k) * st + 8 * c);
+            if (k0 + r >= 0 && k0 + r < n && c < chunks) v[r] = *(const u32x4v*)(x + (int64_t)(k0 + r) * st + 8 * c);
             else v[r] = u32x4v{0, 0, 0, 0};
         }
     };
-    const int items = groups * wchunks;
-    constexpr int HOLD = 2;                    // items per thread that stay in registers between the two passes
-    u32x4v held[HOLD][4];
-    unsigned largest = 0;
-    const auto look = [&](const u32x4v (&v)[4]) {
+    const auto look = [&](const u32x4v (&v)[4], u16x2 m) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) m = __builtin_elementwise_max(m, __builtin_bit_cast(u16x2, v[r][q] & 0x7fff7fffu));
+        return m;
+    };
+    const auto look_finite = [&](const u32x4v (&v)[4], u16x2 m) {
 #pragma unroll
         for (int r = 0; r < 4; ++r)
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
                 const unsigned lo = v[r][q] & 0x7fffu, hi = (v[r][q] >> 16) & 0x7fffu;
-                if (lo < Bits<T>::top && lo > largest) largest = lo;
-                if (hi < Bits<T>::top && hi > largest) largest = hi;
+                m[0] = lo < Bits<T>::top && lo > m[0] ? lo : m[0];
+                m[1] = hi < Bits<T>::top && hi > m[1] ? hi : m[1];
             }
+        return m;
     };
-    int g, c;
+    constexpr int HOLD = 2;                    // items per thread that stay in registers between the two passes
+    u32x4v held[HOLD][4];
+    const auto over_all = [&](auto f) {
+        u16x2 m = {0, 0};
+#pragma unroll
+        for (int h = 0; h < HOLD; ++h)
+            if (tid + h * NT < items) m = f(held[h], m);
+        for (int i = tid + HOLD * NT; i < items; i += NT) {
+            u32x4v v[4];
+            load(i, v);
+            m = f(v, m);
+        }
+        unsigned largest = wave_max(m[0] > m[1] ? m[0] : m[1]);
+        if constexpr (NT == 256) {
+            if ((threadIdx.x & 63) == 0) shared_max[threadIdx.x >> 6] = largest;
+            __syncthreads();
+            largest = max(max(shared_max[0], shared_max[1]), max(shared_max[2], shared_max[3]));
+            __syncthreads();
+        }
+        return (unsigned)__builtin_amdgcn_readfirstlane((int)largest);
+    };
 #pragma unroll
     for (int h = 0; h < HOLD; ++h)
-        if (tid + h * NT < items) { load(tid + h * NT, held[h], g, c); look(held[h]); }
-    for (int i = tid + HOLD * NT; i < items; i += NT) {
-        u32x4v v[4];
-        load(i, v, g, c);
-        look(v);
-    }
-    largest = wave_max(largest);
-    if constexpr (NT == 256) {
-        if ((threadIdx.x & 63) == 0) shared_max[threadIdx.x >> 6] = largest;
-        __syncthreads();
-        largest = max(max(shared_max[0], shared_max[1]), max(shared_max[2], shared_max[3]));
-    }
+        if (tid + h * NT < items) load(tid + h * NT, held[h]);
+    unsigned largest = over_all(look);
+    const bool finite = largest < Bits<T>::top;
+    if (!finite) largest = over_all(look_finite);
     const float wanted = wanted_scale(Bits<T>::f(largest));
     const float now = off == 0 ? wanted : old > wanted ? old : wanted;
     if (off != 0 && now != old) {              // (uniform over the NT threads)
@@ -279,43 +329,38 @@ __device__ __forceinline__ void append_run(const AppendParams& p, int t0, int n,
             *(u32x4v*)(tile + 16 * i) = w;
         }
         __threadfence();                       // these stores are done before the run's own bytes are written
+        if constexpr (NT == 256) __syncthreads();
     }
-    if constexpr (NT == 256) __syncthreads();  // everyone has read the old scale, the rescaled block is written
-    if (tid == 0) *scale = now;
-    const float inv = __builtin_bit_cast(float, (254u << 23) - __builtin_bit_cast(unsigned, now));   // 1 / 2^e
-    const bool pow2 = (__builtin_bit_cast(unsigned, now) & 0x807fffffu) == 0u && now < 0x1p126f;
+    if (tid == 0) *scale = now;                // (everyone has read the old one: it went into the maximum's round)
+    // a power of two that the conversion takes, and nothing but finite values
+    const unsigned nb = __builtin_bit_cast(unsigned, now);
+    const bool fast = finite && (nb & 0x807fffffu) == 0u && nb != 0u && nb != 0x7f800000u;
     const auto put = [&](int i, const u32x4v (&v)[4]) {
-        int gg, cc;
-        if (KEYS) { gg = g0 + i / wchunks; cc = i % wchunks; }
-        else { gg = g0 + i % groups; cc = i / groups; }
-        u32x2 code[4];                         // row r: eight columns
+        int g, c;
+        place(i, g, c);
+        unsigned code[2][4];                   // [four columns][row]
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
+        for (int r = 0; r < 4; ++r)
 #pragma unroll
             for (int q = 0; q < 2; ++q) {
-                unsigned w = 0;
-#pragma unroll
-                for (int z = 0; z < 2; ++z) {
-                    const unsigned u = v[r][2 * q + z];
-                    const float a = Bits<T>::f(u & 0xffffu), b = Bits<T>::f(u >> 16);
-                    w |= (pow2 ? codes2(a * inv, b * inv) : codes2(a / now, b / now)) << (16 * z);
-                }
-                code[r][q] = w;
+                const unsigned a = v[r][2 * q], b = v[r][2 * q + 1];
+                if (fast) code[q][r] = Bits<T>::codes(a, b, now);
+                else code[q][r] = codes2(Bits<T>::f(a & 0xffffu) / now, Bits<T>::f(a >> 16) / now) |
+                                  codes2(Bits<T>::f(b & 0xffffu) / now, Bits<T>::f(b >> 16) / now) << 16;
             }
-        }
-        const int first = 4 * gg - off;        // run index of the group's first position
+        const int first = 4 * g - off;         // run index of the group's first position
         if (KEYS) {
 #pragma unroll
             for (int r = 0; r < 4; ++r)
-                if (first + r >= 0 && first + r < n) *(u32x2*)(tile + (4 * gg + r) * W + 8 * cc) = code[r];
+                if (first + r >= 0 && first + r < n) *(u32x2*)(tile + (4 * g + r) * W + 8 * c) = u32x2{code[0][r], code[1][r]};
         } else {
+            transpose4(code[0]);
+            transpose4(code[1]);
             const bool whole = first >= 0 && first + 4 <= n;
 #pragma unroll
             for (int col = 0; col < 8; ++col) {
-                const int q = col >> 2, b = (col & 3) * 8;
-                const unsigned w = ((code[0][q] >> b) & 0xffu) | ((code[1][q] >> b) & 0xffu) << 8 | ((code[2][q] >> b) & 0xffu) << 16 |
-                                   ((code[3][q] >> b) & 0xffu) << 24;
-                uint8_t* to = tile + (8 * cc + col) * P + 4 * gg;
+                const unsigned w = code[col >> 2][col & 3];
+                uint8_t* to = tile + (8 * c + col) * P + 4 * g;
                 if (whole) *(unsigned*)to = w;
                 else {
 #pragma unroll
@@ -330,67 +375,52 @@ __device__ __forceinline__ void append_run(const AppendParams& p, int t0, int n,
         if (tid + h * NT < items) put(tid + h * NT, held[h]);
     for (int i = tid + HOLD * NT; i < items; i += NT) {
         u32x4v v[4];
-        load(i, v, g, c);
+        load(i, v);
         put(i, v);
     }
-    if constexpr (NT == 256) __syncthreads();  // shared_max is free again
 }
 
-template <typename T>
+template <typename T, int W>
 __global__ __launch_bounds__(256) void cache_append_kernel(AppendParams p) {
-    __shared__ int run_first[64], run_len[64], run_count;
     __shared__ unsigned shared_max[4];
-    const int lane = (int)threadIdx.x & 63, wave = (int)threadIdx.x >> 6;
+    const int lane = (int)threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
     const int head = (int)blockIdx.y >> 1;
     const bool keys = ((int)blockIdx.y & 1) == 0;
     const int P = 1 << p.shift, t_first = (int)blockIdx.x * p.window;
-    // the runs that begin in the window: a token begins one unless its slot follows its predecessor's inside a block
-    if (wave == 0) {
-        const int t = t_first + lane;
-        int slot = -1;
-        bool begins = false;
-        if (lane < p.window && t < p.T) {
-            slot = p.slots[t];
-            if (slot >= 0 && slot < p.limit) {
-                const int prev = t ? p.slots[t - 1] : -2;
-                begins = prev < 0 || prev + 1 != slot || (slot & (P - 1)) == 0;
-            }
-        }
-        const unsigned long long m = __ballot(begins);
-        if (begins) run_first[__popcll(m & ((1ull << lane) - 1))] = t;
-        if (lane == 0) run_count = __popcll(m);
+    // Every wave finds the window's runs by itself, from loads that are in flight together: for the window's tokens and the 128 behind them, whether a
+    // token goes on from its predecessor; a token with a place that does not begins a run, and the ones behind its bit are its length (P <= 128).
+    bool place[3], on[3];
+#pragma unroll
+    for (int i = 0; i < 3; ++i) {
+        const int t = t_first + 64 * i + lane;
+        const int slot = t < p.T ? p.slots[t] : -1, prev = t > 0 && t < p.T ? p.slots[t - 1] : -2;
+        place[i] = slot >= 0 && slot < p.limit;
+        on[i] = place[i] && prev >= 0 && prev + 1 == slot && (slot & (P - 1)) != 0;
     }
-    __syncthreads();
-    const int runs = run_count;
-    if (runs == 0) return;
-    // their lengths: up to the end of the block
-    for (int r = wave; r < runs; r += 4) {
-        const int t0 = run_first[r], slot = p.slots[t0], room = P - (slot & (P - 1));
-        int n = 0;
-        for (int at = 0; at < room; at += 64) {
-            const int k = at + lane;
-            const bool same = k < room && t0 + k < p.T && p.slots[t0 + k] == slot + k;
-            const unsigned long long m = __ballot(same);
-            const int ones = ~m ? __builtin_ctzll(~m) : 64;
-            n += ones;
-            if (ones < 64) break;
+    unsigned long long begins = __ballot(place[0] && !on[0] && lane < p.window);
+    const unsigned long long on0 = __ballot(on[0]), on1 = __ballot(on[1]), on2 = __ballot(on[2]);
+    // one or two runs in a window of 16 tokens and more are long: the whole workgroup takes them; else a wave per run
+    const bool together = p.window >= 16 && __popcll(begins) <= 2;
+    for (int r = 0; begins; ++r) {
+        const int i = __builtin_ctzll(begins);
+        begins &= begins - 1;
+        if (!together && (r & 3) != wave) continue;
+        const auto ones = [](unsigned long long m) { return ~m ? (int)__builtin_ctzll(~m) : 64; };
+        int n = 1 + (i < 63 ? min(ones(on0 >> (i + 1)), 63 - i) : 0);
+        if (n == 64 - i) {
+            const int more = ones(on1);
+            n += more;
+            if (more == 64) n += ones(on2);
         }
-        if (lane == 0) run_len[r] = n;
-    }
-    __syncthreads();
-    // one or two runs in a window of 16 tokens and more are long: the whole workgroup; else a wave per run
-    const bool together = p.window >= 16 && runs <= 2;
-    for (int r = together ? 0 : wave; r < runs; r += together ? 1 : 4) {
-        const int t0 = __builtin_amdgcn_readfirstlane(run_first[r]), n = __builtin_amdgcn_readfirstlane(run_len[r]);
-        const int slot = __builtin_amdgcn_readfirstlane(p.slots[t0]);
+        const int t0 = t_first + i, slot = __builtin_amdgcn_readfirstlane(p.slots[t0]);
         const int64_t block = slot >> p.shift;
         const int off = slot & (P - 1);
         if (together) {
-            if (keys) append_run<T, true, 256>(p, t0, n, block, off, head, shared_max);
-            else append_run<T, false, 256>(p, t0, n, block, off, head, shared_max);
+            if (keys) append_run<T, W, true, 256>(p, t0, n, block, off, head, shared_max);
+            else append_run<T, W, false, 256>(p, t0, n, block, off, head, shared_max);
         } else {
-            if (keys) append_run<T, true, 64>(p, t0, n, block, off, head, shared_max);
-            else append_run<T, false, 64>(p, t0, n, block, off, head, shared_max);
+            if (keys) append_run<T, W, true, 64>(p, t0, n, block, off, head, shared_max);
+            else append_run<T, W, false, 64>(p, t0, n, block, off, head, shared_max);
         }
     }
 }
@@ -406,7 +436,12 @@ hipError_t launch_cache_tables(const TablesParams& p, hipStream_t stream) {
 
 hipError_t launch_cache_append(const AppendParams& p, int dtype, hipStream_t stream) {
     const dim3 grid((unsigned)((p.T + p.window - 1) / p.window), (unsigned)(2 * p.H));
-    return launch1(dtype == 0 ? (const void*)cache_append_kernel<_Float16> : (const void*)cache_append_kernel<__bf16>, grid, dim3(256), 0, stream, p);
+    const auto kernel = [&](auto t) {
+        using T = decltype(t);
+        return p.W == 64 ? (const void*)cache_append_kernel<T, 64> : p.W == 128 ? (const void*)cache_append_kernel<T, 128>
+             : p.W == 192 ? (const void*)cache_append_kernel<T, 192> : (const void*)cache_append_kernel<T, 256>;
+    };
+    return launch1(dtype == 0 ? kernel(_Float16{}) : kernel(__bf16{}), grid, dim3(256), 0, stream, p);
 }
 
 }  // namespace fa
