@@ -93,6 +93,7 @@ struct CacheAttnParams {
     int32_t num_blocks, B, T, Hq, Hkv, group, D, width, shift;
     int32_t grid;           // workgroups of the row kernel
     int32_t min_units;      // fewest 64-token units that are worth a workgroup
+    int32_t whole;          // row kernel: no row tile is cut, none is joined
     int32_t splits;         // tile kernel: parts of a tile's key range
     int32_t max_tiles;      // tile kernel: bound on the row tiles of one key/value head
     float scale_log2;
@@ -101,7 +102,7 @@ struct CacheAttnPlan {
     int32_t tile;           // 0 = row kernel (few query rows per key/value head), 1 = tile kernel
     int32_t nr;             // 16-row query tiles per wave
     int32_t width;          // W
-    int32_t grid, splits, max_tiles, min_units;
+    int32_t grid, splits, max_tiles, min_units, whole;
     int64_t ws_o, ws_ml, ws_prefix, bytes;   // workspace offsets in bytes and its size
 };
 hipError_t launch_cache_attn(const CacheAttnParams& p, const CacheAttnPlan& plan, int dtype, hipStream_t stream);

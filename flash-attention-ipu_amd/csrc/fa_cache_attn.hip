@@ -10,9 +10,10 @@
 //   * row `r` of key tile t (16 keys) is key 16 (r >> 2) + 4 t + (r & 3) of the unit: a lane's four results of the four tiles are the sixteen
 //     CONSECUTIVE keys 16 (lane >> 4) .. + 15, which is what the B operand of the second product wants of that lane (two products of 32 keys);
 //   * the value cache is token-inner, so the matching A operand (column d, those sixteen keys) is one 16-byte load, as is a key row's share.
-// e4m3 -> 16-bit is exact, one instruction per two values.  A unit's products of codes start from zero and are added as O += scale_v acc: the
-// scale multiplies in 32 bits, and P <= 1 is rounded once to the operand type as in the kernels for 16-bit operands.  Blocks shorter than a
-// unit bring several value scales into one product: P is then multiplied by scale_v / (largest scale_v of the unit) before it is rounded.
+// e4m3 -> 16-bit is exact, one instruction per two values.  Scales cost no instruction per score: scale_k and the softmax scale are the factor
+// of the exponent's fma, and the weight that meets the codes of V is P' = P scale_v / ref = 2^(s kf - (max - log2(scale_v / ref))), rounded once to
+// the operand type; the sum of the weights takes a lane's sum of P' times ref / scale_v, once per unit.  ref: 1 for bf16, whose exponents reach as
+// far as 32-bit ones; for f16 a reference that follows the scales and keeps the weights between its subnormals and its largest value.
 // Maximum, sum and O are 32-bit.
 //
 // Two kernels:
@@ -187,22 +188,26 @@ struct RowState {
     static constexpr int NC = W / 32, ND = W / 16;       // k-steps of Q K^T; 16-column tiles of O
     using vec8 = typename Elt<T>::vec8;
     vec8 q[NR][NC];
-    float o[NR][ND][4];                                  // (scalars: as vectors, every conditional change copies them)
+    f32x4 o[NR][ND];
+    float ref;                                           // f16: O is in units of this value scale (uniform; 0 = none yet), and the largest it was
+    float ref_max;
     float m[NR], l[NR];
     int limit[NR];                                       // keys that the lane's row sees
     int limit_min, limit_max;                            // over the wave's rows (uniform)
     unsigned long long nan[NR];                          // bit 4 d + i: o[r][d][i] saw a NaN value (note_nan)
 
+    static constexpr bool kRef = Elt<T>::is_f16;
+
     __device__ __forceinline__ void clear() {
+        ref = kRef ? 0.f : 1.f;
+        ref_max = ref;
 #pragma unroll
         for (int r = 0; r < NR; ++r) {
             m[r] = -INFINITY;
             l[r] = 0.f;
             nan[r] = 0;
 #pragma unroll
-            for (int d = 0; d < ND; ++d)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) o[r][d][i] = 0.f;
+            for (int d = 0; d < ND; ++d) o[r][d] = f32x4{0.f, 0.f, 0.f, 0.f};
         }
     }
     // rows row0 .. row0 + 16 NR - 1 of (request, key/value head h)
@@ -227,9 +232,9 @@ struct RowState {
             }
         }
     }
-    // key(t, c): fragment c of key tile t; value(d, u): fragment of columns 16 d .., keys 8 u .. + 7 of every lane's sixteen.  kf: scale_k times the softmax
-    // scale in powers of two, and dead: whether the lane's sixteen keys are masked altogether; vs: the unit's value scale, ratio: the lane's share of it
-    template <typename Key>
+    // S^T of a unit.  key(t, c): fragment c of key tile t.  FENCE: key tiles one after the other - where `key` converts, the compiler would otherwise
+    // convert all of them first and spill
+    template <bool FENCE, typename Key>
     __device__ __forceinline__ void scores(Key key, f32x4 (&s)[NR][4]) const {
 #pragma unroll
         for (int t = 0; t < 4; ++t) {
@@ -241,38 +246,53 @@ struct RowState {
 #pragma unroll
                 for (int r = 0; r < NR; ++r) s[r][t] = Elt<T>::mfma16(a, q[r][c], s[r][t]);
             }
-            __builtin_amdgcn_sched_barrier(0);           // (else every tile's conversions are hoisted and the registers spill)
+            if (FENCE) __builtin_amdgcn_sched_barrier(0);
         }
     }
-    template <bool SMALL>
-    __device__ __forceinline__ void softmax(f32x4 (&s)[NR][4], vec8 (&w)[NR][2], int key0, float kf, bool dead, float ratio, bool boundary) {
+    // f16: weights P' = P scale_v / ref stay below 2^13 and, where P is not small against its row's largest, above 2^-14.  top: the unit's largest value scale.
+    // ref goes down to 2^-40 of the largest it was: values of scales far below that vanish beside the others, and O in units of ref stays finite
+    __device__ __forceinline__ void follow(float top) {
+        if constexpr (kRef) {
+            const float low = ref_max * 0x1p-40f;
+            if (top > ref * 8192.f || (top * 8.f < ref && ref > low)) {       // (uniform)
+                const float now = __builtin_fmaxf(top * 0x1p-6f, low), f = ref / now;
+#pragma unroll
+                for (int r = 0; r < NR; ++r)
+#pragma unroll
+                    for (int d = 0; d < ND; ++d) o[r][d] *= f;
+                ref = now;
+                ref_max = __builtin_fmaxf(ref_max, now);
+            }
+        }
+    }
+    // P' of a unit.  kf: scale_k times the softmax scale in powers of two; vs: the lane's value scale; dead: its sixteen keys (from key0 on) have no block
+    __device__ __forceinline__ void softmax(f32x4 (&s)[NR][4], vec8 (&w)[NR][2], int key0, float kf, float vs, bool dead, bool masked) {
+        const float shift = __builtin_amdgcn_logf(kRef ? vs * __builtin_amdgcn_rcpf(ref) : vs);
+        const float back = kRef ? ref * __builtin_amdgcn_rcpf(vs) : __builtin_amdgcn_rcpf(vs);
 #pragma unroll
         for (int r = 0; r < NR; ++r) {
-            float top = -INFINITY;
-#pragma unroll
-            for (int t = 0; t < 4; ++t) s[r][t] *= kf;
-            if (boundary || SMALL) {
-                const int see = dead ? 0 : limit[r] - key0;        // the lane's keys are key0 .. key0 + 15
+            if (masked) {
+                const int see = dead ? 0 : limit[r] - key0;
 #pragma unroll
                 for (int t = 0; t < 4; ++t)
 #pragma unroll
                     for (int i = 0; i < 4; ++i) s[r][t][i] = 4 * t + i < see ? s[r][t][i] : -INFINITY;
             }
+            float top = -INFINITY;
 #pragma unroll
             for (int t = 0; t < 4; ++t)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) top = __builtin_fmaxf(top, s[r][t][i]);
-            top = rows_max(top);
-            const float now = __builtin_fmaxf(m[r], top), base = now == -INFINITY ? 0.f : now;
+                for (int i = 0; i < 4; i += 2) top = __builtin_fmaxf(__builtin_fmaxf(top, s[r][t][i]), s[r][t][i + 1]);
+            top = rows_max(top * kf);
+            const float now = __builtin_fmaxf(m[r], top);
             if (__any(now > m[r])) {
-                const float alpha = fast_exp2(m[r] - base);
+                const float alpha = fast_exp2(m[r] - (now == -INFINITY ? 0.f : now));
                 l[r] *= alpha;
 #pragma unroll
-                for (int d = 0; d < ND; ++d)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) o[r][d][i] *= alpha;
+                for (int d = 0; d < ND; ++d) o[r][d] *= alpha;
                 m[r] = now;
             }
+            const float base = shift - (now == -INFINITY ? 0.f : now);
             float sum = 0.f;
             unsigned u[8];
 #pragma unroll
@@ -280,37 +300,42 @@ struct RowState {
                 float e[4];
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    e[i] = fast_exp2(s[r][t][i] - base);
+                    e[i] = fast_exp2(__builtin_fmaf(s[r][t][i], kf, base));
                     sum += e[i];
-                    if constexpr (SMALL) e[i] *= ratio;
                 }
                 u[2 * t] = pack2<T>(e[0], e[1]);
                 u[2 * t + 1] = pack2<T>(e[2], e[3]);
             }
-            l[r] += sum;
+            l[r] = __builtin_fmaf(sum, back, l[r]);
             const u32x4 a = {u[0], u[1], u[2], u[3]}, b = {u[4], u[5], u[6], u[7]};
             w[r][0] = __builtin_bit_cast(vec8, a);
             w[r][1] = __builtin_bit_cast(vec8, b);
         }
     }
-    template <int D0, int D1, typename Value>
-    __device__ __forceinline__ void values(Value value, const vec8 (&w)[NR][2], float vs) {
-        const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
-        __builtin_amdgcn_sched_barrier(0);
+    // O^T += V^T P'^T for the column tiles D0 .. D1 - 1.  value(d, u): fragment of columns 16 d .., keys 8 u .. + 7 of every lane's sixteen
+    template <int D0, int D1, bool FENCE, typename Value>
+    __device__ __forceinline__ void values(Value value, const vec8 (&w)[NR][2]) {
+        if (FENCE) __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int d = D0; d < D1; ++d) {
-            const vec8 a = value(d, 0), b = value(d, 1);
 #pragma unroll
-            for (int r = 0; r < NR; ++r) {
-                f32x4 acc = Elt<T>::mfma16(a, w[r][0], zero);
-                acc = Elt<T>::mfma16(b, w[r][1], acc);
+            for (int u = 0; u < 2; ++u) {
+                const vec8 a = value(d, u);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) o[r][d][i] = __builtin_fmaf(acc[i], vs, o[r][d][i]);
-                // (pinned here: the compiler moves these sums behind the loop's last branch and keeps every product's registers until then)
-                asm volatile("" : "+v"(o[r][d][0]), "+v"(o[r][d][1]), "+v"(o[r][d][2]), "+v"(o[r][d][3]));
+                for (int r = 0; r < NR; ++r) o[r][d] = Elt<T>::mfma16(a, w[r][u], o[r][d]);
             }
-            if (NR * W > 128 || d % 2) __builtin_amdgcn_sched_barrier(0);
+            if (FENCE && (NR * W > 128 || d % 2)) __builtin_amdgcn_sched_barrier(0);
         }
+    }
+    // the segment's end: O in plain units, NaN where it was seen
+    __device__ __forceinline__ void finish() {
+        if constexpr (kRef) {
+#pragma unroll
+            for (int r = 0; r < NR; ++r)
+#pragma unroll
+                for (int d = 0; d < ND; ++d) o[r][d] *= ref;
+        }
+        put_nan();
     }
     // A unit that some rows see only in part holds NaN values: they were taken out of the operands (take_nan) and are noted for the rows that see
     // them; keys[column]: the unit's keys with NaN in that column
@@ -351,8 +376,8 @@ struct RowState {
             for (int d = 0; d < ND; ++d) {
                 const int at = 16 * d + 4 * lg;
                 if (at >= p.D) continue;
-                const float* v = o[r][d];
-                *(u32x2c*)(dst + at) = u32x2c{pack2<T>(v[0] * inv, v[1] * inv), pack2<T>(v[2] * inv, v[3] * inv)};
+                const f32x4 v = o[r][d] * inv;
+                *(u32x2c*)(dst + at) = u32x2c{pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3])};
             }
         }
     }
@@ -364,7 +389,7 @@ struct RowState {
             const long long row = slot * rows16 + at + 16 * r + col;
             if (lg == 0) { p.ws_ml[2 * row] = top[r]; p.ws_ml[2 * row + 1] = sum[r]; }
 #pragma unroll
-            for (int d = 0; d < ND; ++d) *(f32x4*)(p.ws_o + row * W + 16 * d + 4 * lg) = f32x4{o[r][d][0], o[r][d][1], o[r][d][2], o[r][d][3]};
+            for (int d = 0; d < ND; ++d) *(f32x4*)(p.ws_o + row * W + 16 * d + 4 * lg) = o[r][d];
         }
     }
 };
@@ -381,8 +406,11 @@ template <bool SMALL>
 struct UnitAt {
     const uint8_t* k;
     const uint8_t* v;
-    float kf, vs, ratio;
+    float kf, vs, top;        // the lane's factors (softmax()), the unit's largest value scale
     bool dead, none;          // the lane's sixteen keys have no block; the unit has none at all (uniform)
+    bool blank;               // their values count as zeros: no block, or a scale of zero
+    // (a scale of zero, or none, becomes one that makes everything vanish but leaves no 0 * inf)
+    static __device__ __forceinline__ float factor(float x) { return __builtin_fmaxf(x, 0x1p-100f); }
     __device__ __forceinline__ void find(const CacheAttnParams& p, const int* table, int len, int u, int h, int W, int lane) {
         const int lg = lane >> 4, wk = lane & 15, P = 1 << p.shift, first = 64 * u;
         if constexpr (!SMALL) {
@@ -393,9 +421,11 @@ struct UnitAt {
             const int in = first & (P - 1);
             k = p.k + blk * p.k_bs + (int64_t)(h * P + in) * W;
             v = p.v + blk * p.v_bs + (int64_t)h * P * W + in;
-            kf = none ? 0.f : p.ks[blk * p.ks_bs + h] * p.scale_log2;
+            kf = factor(none ? 0.f : p.ks[blk * p.ks_bs + h] * p.scale_log2);
             vs = none ? 0.f : p.vs[blk * p.vs_bs + h];
-            ratio = 1.f;
+            blank = vs == 0.f;
+            vs = factor(vs);
+            top = vs;
         } else {
             const int kk = first + 16 * (wk >> 2), vk = first + 16 * lg;
             const int kid = kk < len ? block_at(p, table, kk >> p.shift) : -1;
@@ -405,10 +435,11 @@ struct UnitAt {
             const long long kb = kid < 0 ? 0 : kid, vb = vid < 0 ? 0 : vid;
             k = p.k + kb * p.k_bs + (int64_t)(h * P + (kk & (P - 1))) * W;
             v = p.v + vb * p.v_bs + (int64_t)h * P * W + (vk & (P - 1));
-            kf = dead ? 0.f : p.ks[vb * p.ks_bs + h] * p.scale_log2;
-            const float mine = dead ? 0.f : p.vs[vb * p.vs_bs + h];
-            vs = rows_max(mine);
-            ratio = vs > 0.f ? mine / vs : 0.f;
+            kf = factor(dead ? 0.f : p.ks[vb * p.ks_bs + h] * p.scale_log2);
+            vs = dead ? 0.f : p.vs[vb * p.vs_bs + h];
+            blank = vs == 0.f;
+            vs = factor(vs);
+            top = rows_max(vs);
         }
     }
     // byte offset of key tile 0's row of this lane, and of its row of value column 0
@@ -422,9 +453,10 @@ struct UnitAt {
 };
 
 // ---- row kernel ---------------------------------------------------------------------------------------------------------------------------
+// (whole: the line is made of row tiles, none of which is cut)
 __device__ __forceinline__ long long row_items(const CacheAttnParams& p, const Request& rq, int rows16) {
     const int tiles = (rq.n * p.group + rows16 - 1) / rows16;
-    return (long long)tiles * p.Hkv * rq.units;
+    return (long long)tiles * p.Hkv * (p.whole ? 1 : rq.units);
 }
 __device__ __forceinline__ long long range_of(const CacheAttnParams& p, long long total) {
     const long long per = (total + p.grid - 1) / p.grid;
@@ -438,7 +470,7 @@ __global__ __launch_bounds__(256, 2) void cache_rows_kernel(CacheAttnParams p) {
     // the next unit's codes are fetched under this one's arithmetic where the registers hold them beside O; else a unit's value columns are
     // taken in parts
     constexpr bool AHEAD = W * NR <= 128;
-    constexpr int VN = AHEAD ? ND : W > 192 && SMALL ? ND / 8 : W * NR > 192 ? ND / 4 : ND / 2;
+    constexpr int VN = AHEAD ? ND : W > 192 ? ND / 8 : W * NR > 192 ? ND / 4 : ND / 2;
     __shared__ __align__(8) unsigned short nan_keys[4][4 * W];     // [wave][column][16-key group]
     __shared__ f32x4 join_o[2][NR * ND * 64];
     __shared__ float join_m[4][ROWS], join_l[4][ROWS];
@@ -457,11 +489,12 @@ __global__ __launch_bounds__(256, 2) void cache_rows_kernel(CacheAttnParams p) {
     while (cur < end) {
         const Request rq = request_of(p, b);
         const int tiles = (rq.n * p.group + ROWS - 1) / ROWS;
-        const long long items = (long long)tiles * p.Hkv * rq.units;
+        const int per = p.whole ? 1 : rq.units;            // items of a row tile
+        const long long items = (long long)tiles * p.Hkv * per;
         if (off >= items) { ++b; off = 0; continue; }      // (the next request with rows; there is one, cur < end)
-        const int ht = (int)(off / rq.units), u0 = (int)(off - (long long)ht * rq.units);
+        const int ht = (int)(off / per), u0 = (int)(off - (long long)ht * per);
         const int h = ht / tiles, row0 = (ht - h * tiles) * ROWS;
-        const int u1 = (int)(u0 + (end - cur) < rq.units ? u0 + (end - cur) : rq.units);
+        const int u1 = p.whole || u0 + (end - cur) >= rq.units ? rq.units : (int)(u0 + (end - cur));
         const bool whole = u0 == 0 && u1 == rq.units;
         const int* table = p.tables + (int64_t)b * p.table_stride;
         st.load(p, rq, h, row0, lane);
@@ -499,16 +532,17 @@ __global__ __launch_bounds__(256, 2) void cache_rows_kernel(CacheAttnParams p) {
                 const int key0 = 64 * u + 16 * lg;
                 f32x4 s[NR][4];
                 typename State::vec8 w[NR][2];
-                st.scores([&](int t, int c) { return fragment<T>(kr[t][c >> 1][2 * (c & 1)], kr[t][c >> 1][2 * (c & 1) + 1]); }, s);
+                st.template scores<true>([&](int t, int c) { return fragment<T>(kr[t][c >> 1][2 * (c & 1)], kr[t][c >> 1][2 * (c & 1) + 1]); }, s);
                 if (!AHEAD) load_values(here, 0);
                 else if (more) load_keys(next);
                 else drop_keys();
-                st.template softmax<SMALL>(s, w, key0, here.kf, here.dead, here.ratio, boundary);
+                st.follow(here.top);
+                st.softmax(s, w, key0, here.kf, here.vs, here.dead, boundary || (SMALL && __any(here.dead)));
                 bool nan = false;
                 const auto part = [&](auto from) {
                     constexpr int D0 = decltype(from)::value;
-                    if (64 * u + 64 > rq.len || __any(here.dead)) {
-                        const int valid = here.dead ? 0 : rq.len - key0;
+                    if (64 * u + 64 > rq.len || __any(here.blank)) {
+                        const int valid = here.blank ? 0 : rq.len - key0;
 #pragma unroll
                         for (int d = 0; d < VN; ++d) vr[d] = clear_behind(vr[d], valid);
                     }
@@ -530,7 +564,7 @@ __global__ __launch_bounds__(256, 2) void cache_rows_kernel(CacheAttnParams p) {
                             }
                         }
                     }
-                    st.template values<D0, D0 + VN>([&](int d, int v) { return fragment<T>(vr[d - D0][2 * v], vr[d - D0][2 * v + 1]); }, w, here.vs);
+                    st.template values<D0, D0 + VN, true>([&](int d, int v) { return fragment<T>(vr[d - D0][2 * v], vr[d - D0][2 * v + 1]); }, w);
                 };
                 fa_static_for<0, ND / VN>([&](auto i) {
                     if constexpr (decltype(i)::value > 0) load_values(here, decltype(i)::value * VN);
@@ -546,7 +580,7 @@ __global__ __launch_bounds__(256, 2) void cache_rows_kernel(CacheAttnParams p) {
         }
         // the waves' parts joined, the first wave ends with the sums
         const int active = min(4, u1 - u0);
-        st.put_nan();
+        st.finish();
     float sum[NR], top[NR];
 #pragma unroll
         for (int r = 0; r < NR; ++r) { sum[r] = rows_sum(st.l[r]); top[r] = st.m[r]; }
@@ -566,9 +600,7 @@ __global__ __launch_bounds__(256, 2) void cache_rows_kernel(CacheAttnParams p) {
                 for (int w = 0; w < 4; ++w) total += join_l[w][16 * r + wk] * fast_exp2(join_m[w][16 * r + wk] - base);
                 const float f = fast_exp2(top[r] - base);
 #pragma unroll
-                for (int d = 0; d < ND; ++d)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) st.o[r][d][i] *= f;
+                for (int d = 0; d < ND; ++d) st.o[r][d] *= f;
                 top[r] = all;
                 sum[r] = total;
             }
@@ -578,18 +610,14 @@ __global__ __launch_bounds__(256, 2) void cache_rows_kernel(CacheAttnParams p) {
 #pragma unroll
                     for (int r = 0; r < NR; ++r)
 #pragma unroll
-                        for (int d = 0; d < ND; ++d) join_o[wave - step][(r * ND + d) * 64 + lane] = f32x4{st.o[r][d][0], st.o[r][d][1], st.o[r][d][2], st.o[r][d][3]};
+                        for (int d = 0; d < ND; ++d) join_o[wave - step][(r * ND + d) * 64 + lane] = st.o[r][d];
                 }
                 __syncthreads();
                 if (wave < step) {
 #pragma unroll
                     for (int r = 0; r < NR; ++r)
 #pragma unroll
-                        for (int d = 0; d < ND; ++d) {
-                            const f32x4 v = join_o[wave][(r * ND + d) * 64 + lane];
-#pragma unroll
-                            for (int i = 0; i < 4; ++i) st.o[r][d][i] += v[i];
-                        }
+                        for (int d = 0; d < ND; ++d) st.o[r][d] += join_o[wave][(r * ND + d) * 64 + lane];
                 }
                 __syncthreads();
             }
@@ -598,8 +626,8 @@ __global__ __launch_bounds__(256, 2) void cache_rows_kernel(CacheAttnParams p) {
             if (whole) st.store(p, rq, h, row0, lane, sum);
             else st.park(p, 2ll * blockIdx.x + (cur == start ? 0 : 1), ROWS, 0, lane, sum, top);
         }
-        cur += u1 - u0;
-        off += u1 - u0;
+        cur += p.whole ? 1 : u1 - u0;
+        off += p.whole ? 1 : u1 - u0;
     }
 }
 
@@ -656,8 +684,8 @@ __global__ __launch_bounds__(256, W > 128 ? 1 : 2) void cache_tile_kernel(CacheA
 #pragma unroll
             for (int c = 0; c < 2; ++c)
                 lds_k[buf][(wave * NC + 2 * i + c) * 64 + lane] = __builtin_bit_cast(u32x4, fragment<T>(kr[i][2 * c], kr[i][2 * c + 1]));
-        if (64 * u + 64 > rq.len || (SMALL && __any(a.dead))) {
-            const int valid = a.dead ? 0 : rq.len - (64 * u + 16 * lg);
+        if (64 * u + 64 > rq.len || __any(a.blank)) {
+            const int valid = a.blank ? 0 : rq.len - (64 * u + 16 * lg);
 #pragma unroll
             for (int i = 0; i < VPW; ++i) vr[i] = clear_behind(vr[i], valid);
         }
@@ -694,9 +722,10 @@ __global__ __launch_bounds__(256, W > 128 ? 1 : 2) void cache_tile_kernel(CacheA
             const bool boundary = 64 * u + 64 > st.limit_min;
             f32x4 s[NR][4];
             vec8 w[NR][2];
-            st.scores([&](int t, int c) { return __builtin_bit_cast(vec8, lds_k[buf][(t * NC + c) * 64 + lane]); }, s);
-            st.template softmax<SMALL>(s, w, key0, here.kf, here.dead, here.ratio, boundary);
-            st.template values<0, ND>([&](int d, int v) { return __builtin_bit_cast(vec8, lds_v[buf][(d * 2 + v) * 64 + lane]); }, w, here.vs);
+            st.template scores<false>([&](int t, int c) { return __builtin_bit_cast(vec8, lds_k[buf][(t * NC + c) * 64 + lane]); }, s);
+            st.follow(here.top);
+            st.softmax(s, w, key0, here.kf, here.vs, here.dead, boundary || (SMALL && __any(here.dead)));
+            st.template values<0, ND, false>([&](int d, int v) { return __builtin_bit_cast(vec8, lds_v[buf][(d * 2 + v) * 64 + lane]); }, w);
             if (nan_found[buf] == u + 1) st.note_nan((const unsigned long long*)nan_keys[buf], u, lg);
         }
         if (more) {
@@ -705,7 +734,7 @@ __global__ __launch_bounds__(256, W > 128 ? 1 : 2) void cache_tile_kernel(CacheA
         }
         __syncthreads();
     }
-    st.put_nan();
+    st.finish();
     float sum[NR], top[NR];
 #pragma unroll
     for (int r = 0; r < NR; ++r) { sum[r] = rows_sum(st.l[r]); top[r] = st.m[r]; }
@@ -810,7 +839,7 @@ template <typename T>
 hipError_t launch_typed(const CacheAttnParams& p, const CacheAttnPlan& plan, hipStream_t stream) {
     hipError_t e = plan.width == 64 ? launch_width<T, 64>(p, plan, stream) : plan.width == 128 ? launch_width<T, 128>(p, plan, stream)
                  : plan.width == 192 ? launch_width<T, 192>(p, plan, stream) : launch_width<T, 256>(p, plan, stream);
-    if (e != hipSuccess || (plan.tile && plan.splits == 1)) return e;
+    if (e != hipSuccess || (plan.tile ? plan.splits == 1 : p.whole)) return e;
     const int rows16 = (plan.tile ? 64 : 16) * plan.nr;
     CacheAttnParams arg = p;
     int W = plan.width, rows = rows16;

@@ -23,6 +23,7 @@ int launched(hipError_t e) { return e == hipSuccess ? FA_OK : fail(FA_ERR_LAUNCH
 
 constexpr int64_t kMaxCount = 1ll << 30;      // rows, items, tokens: 32-bit indexes with room for a grid's stride
 constexpr int64_t kMaxStride = 1ll << 40;     // elements: products with 32-bit indexes stay inside 64 bits
+constexpr int kWholeUnits = 16;               // 64-token units of a request up to which the row kernel cuts none
 constexpr int kCus = 256;                     // compute units of an MI355X: sizes grids, never correctness
 
 int64_t up(int64_t a, int64_t b) { return (a + b - 1) / b; }
@@ -130,13 +131,17 @@ int attn_plan(int64_t B, int64_t T, int64_t heads, int64_t heads_kv, int64_t D, 
         p.nr = rows > 16 && W <= 128 ? 2 : 1;
         p.max_tiles = (int32_t)up(rows, 16 * p.nr);
         int64_t grid = W > 64 || p.nr > 1 ? 2 * kCus : 3 * kCus;
-        const int64_t most = up(B * heads_kv * p.max_tiles * max_units, p.min_units);
+        // short caches: four waves are through a row's units in a few rounds, which is less than a second launch takes
+        p.whole = max_units <= kWholeUnits;
+        if (p.whole) p.min_units = 1;
+        const int64_t most = p.whole ? B * heads_kv * p.max_tiles : up(B * heads_kv * p.max_tiles * max_units, p.min_units);
         if (grid > most) grid = most;
         p.grid = (int32_t)grid;
         p.splits = 1;
         p.ws_o = 0;
-        p.ws_ml = 2 * grid * 16 * p.nr * W * 4;
-        p.ws_prefix = p.ws_ml + 2 * grid * 16 * p.nr * 8;
+        const int64_t slots = p.whole ? 0 : 2 * grid;
+        p.ws_ml = slots * 16 * p.nr * W * 4;
+        p.ws_prefix = p.ws_ml + slots * 16 * p.nr * 8;
     } else {
         p.nr = W <= 128 ? 2 : 1;
         const int64_t rows_wg = 64 * p.nr, tiles = up(T * group, rows_wg), bound = T * group / rows_wg + B;
@@ -312,7 +317,7 @@ int fa_cache_attn(const void* q, void* out, const void* k_cache, const void* v_c
     p.k_bs = block_strides[0]; p.v_bs = block_strides[1]; p.ks_bs = block_strides[2]; p.vs_bs = block_strides[3]; p.table_stride = table_stride;
     p.num_blocks = (int32_t)num_blocks; p.B = (int32_t)num_requests; p.T = (int32_t)num_tokens; p.Hq = (int32_t)heads; p.Hkv = (int32_t)heads_kv;
     p.group = (int32_t)(heads / heads_kv); p.D = (int32_t)D; p.width = (int32_t)max_blocks; p.shift = block_shift(block_size);
-    p.grid = plan.grid; p.min_units = plan.min_units; p.splits = plan.splits; p.max_tiles = plan.max_tiles;
+    p.grid = plan.grid; p.min_units = plan.min_units; p.whole = plan.whole; p.splits = plan.splits; p.max_tiles = plan.max_tiles;
     p.scale_log2 = softmax_scale * 1.44269504088896340736f;
     return launched(fa::launch_cache_attn(p, plan, dtype, (hipStream_t)stream));
 }

@@ -137,7 +137,7 @@ int main() {
                 CHECK(g_plan.grid == Hk * g_plan.max_tiles * g_plan.splits && g_plan.max_tiles >= (T * group + rows - 1) / rows);
             } else {
                 rows = 16 * g_plan.nr;
-                slots = 2ll * g_plan.grid;
+                slots = g_plan.whole ? 0 : 2ll * g_plan.grid;
                 CHECK(g_plan.nr == 1 || W <= 128);
             }
             CHECK(g_plan.ws_ml - g_plan.ws_o >= slots * rows * W * 4 && g_plan.ws_prefix - g_plan.ws_ml >= slots * rows * 8);
