@@ -194,7 +194,8 @@ struct RowState {
     float m[NR], l[NR];
     int limit[NR];                                       // keys that the lane's row sees
     int limit_min, limit_max;                            // over the wave's rows (uniform)
-    unsigned long long nan[NR];                          // bit 4 d + i: o[r][d][i] saw a NaN value (note_nan)
+    using NanBits = typename std::conditional<W <= 128, unsigned, unsigned long long>::type;
+    NanBits nan[NR];                                     // bit 4 d + i: o[r][d][i] saw a NaN value (note_nan)
 
     static constexpr bool kRef = Elt<T>::is_f16;
 
@@ -249,13 +250,52 @@ struct RowState {
             if (FENCE) __builtin_amdgcn_sched_barrier(0);
         }
     }
-    // f16: weights P' = P scale_v / ref stay below 2^13 and, where P is not small against its row's largest, above 2^-14.  top: the unit's largest value scale.
-    // ref goes down to 2^-40 of the largest it was: values of scales far below that vanish beside the others, and O in units of ref stays finite
+    // scores that a row may not see; the lane's keys are key0 .. key0 + 15, dead: they have no block
+    __device__ __forceinline__ void mask(f32x4 (&s)[NR][4], int key0, bool dead) const {
+#pragma unroll
+        for (int r = 0; r < NR; ++r) {
+            const int see = dead ? 0 : limit[r] - key0;
+#pragma unroll
+            for (int t = 0; t < 4; ++t)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) s[r][t][i] = 4 * t + i < see ? s[r][t][i] : -INFINITY;
+        }
+    }
+    // every row's largest score of the unit, in powers of two.  kf: scale_k times the softmax scale
+    __device__ __forceinline__ void peak(const f32x4 (&s)[NR][4], float kf, float (&top)[NR]) const {
+#pragma unroll
+        for (int r = 0; r < NR; ++r) {
+            float x = -INFINITY;
+#pragma unroll
+            for (int t = 0; t < 4; ++t)
+#pragma unroll
+                for (int i = 0; i < 4; i += 2) x = __builtin_fmaxf(__builtin_fmaxf(x, s[r][t][i]), s[r][t][i + 1]);
+            top[r] = rows_max(x * kf);
+        }
+    }
+    // the reference maximum goes up where a score would leave 2^kSlack above it (weights up to 2^kSlack round as well as weights up to 1); most units do not
+    // pay for the rescale
+    static constexpr float kSlack = 8.f;
+    __device__ __forceinline__ void raise(const float (&top)[NR]) {
+#pragma unroll
+        for (int r = 0; r < NR; ++r) {
+            if (__any(top[r] > m[r] + kSlack)) {
+                const float now = __builtin_fmaxf(m[r], top[r]), alpha = fast_exp2(m[r] - (now == -INFINITY ? 0.f : now));
+                l[r] *= alpha;
+#pragma unroll
+                for (int d = 0; d < ND; ++d) o[r][d] *= alpha;
+                m[r] = now;
+            }
+        }
+    }
+    // f16: scale_v / ref stays in 2^-3 .. 2^7: with P up to 2^kSlack the weights stay below 2^15 and, where P is not small against its row's largest, above
+    // 2^-14.  top: the unit's largest value scale.  ref goes down to 2^-40 of the largest it was: values of scales far below that vanish beside the others, and O
+    // in units of ref stays finite
     __device__ __forceinline__ void follow(float top) {
         if constexpr (kRef) {
             const float low = ref_max * 0x1p-40f;
-            if (top > ref * 8192.f || (top * 8.f < ref && ref > low)) {       // (uniform)
-                const float now = __builtin_fmaxf(top * 0x1p-6f, low), f = ref / now;
+            if (top > ref * 128.f || (top * 8.f < ref && ref > low)) {       // (uniform)
+                const float now = __builtin_fmaxf(top * 0.125f, low), f = ref / now;
 #pragma unroll
                 for (int r = 0; r < NR; ++r)
 #pragma unroll
@@ -265,35 +305,14 @@ struct RowState {
             }
         }
     }
-    // P' of a unit.  kf: scale_k times the softmax scale in powers of two; vs: the lane's value scale; dead: its sixteen keys (from key0 on) have no block
-    __device__ __forceinline__ void softmax(f32x4 (&s)[NR][4], vec8 (&w)[NR][2], int key0, float kf, float vs, bool dead, bool masked) {
+    // P' of a unit, and its sum into l.  vs: the lane's value scale
+    __device__ __forceinline__ void weights(const f32x4 (&s)[NR][4], vec8 (&w)[NR][2], float kf, float vs) {
         const float shift = __builtin_amdgcn_logf(kRef ? vs * __builtin_amdgcn_rcpf(ref) : vs);
         const float back = kRef ? ref * __builtin_amdgcn_rcpf(vs) : __builtin_amdgcn_rcpf(vs);
 #pragma unroll
         for (int r = 0; r < NR; ++r) {
-            if (masked) {
-                const int see = dead ? 0 : limit[r] - key0;
-#pragma unroll
-                for (int t = 0; t < 4; ++t)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) s[r][t][i] = 4 * t + i < see ? s[r][t][i] : -INFINITY;
-            }
-            float top = -INFINITY;
-#pragma unroll
-            for (int t = 0; t < 4; ++t)
-#pragma unroll
-                for (int i = 0; i < 4; i += 2) top = __builtin_fmaxf(__builtin_fmaxf(top, s[r][t][i]), s[r][t][i + 1]);
-            top = rows_max(top * kf);
-            const float now = __builtin_fmaxf(m[r], top);
-            if (__any(now > m[r])) {
-                const float alpha = fast_exp2(m[r] - (now == -INFINITY ? 0.f : now));
-                l[r] *= alpha;
-#pragma unroll
-                for (int d = 0; d < ND; ++d) o[r][d] *= alpha;
-                m[r] = now;
-            }
-            const float base = shift - (now == -INFINITY ? 0.f : now);
-            float sum = 0.f;
+            const float base = shift - (m[r] == -INFINITY ? 0.f : m[r]);
+            float sum[2] = {0.f, 0.f};
             unsigned u[8];
 #pragma unroll
             for (int t = 0; t < 4; ++t) {
@@ -301,12 +320,13 @@ struct RowState {
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     e[i] = fast_exp2(__builtin_fmaf(s[r][t][i], kf, base));
-                    sum += e[i];
+                    sum[i & 1] += e[i];
                 }
                 u[2 * t] = pack2<T>(e[0], e[1]);
                 u[2 * t + 1] = pack2<T>(e[2], e[3]);
             }
-            l[r] = __builtin_fmaf(sum, back, l[r]);
+            l[r] = __builtin_fmaf(sum[0] + sum[1], back, l[r]);
+            asm volatile("" : "+v"(l[r]));            // (here: moved behind the products, the sum would keep every weight in a register)
             const u32x4 a = {u[0], u[1], u[2], u[3]}, b = {u[4], u[5], u[6], u[7]};
             w[r][0] = __builtin_bit_cast(vec8, a);
             w[r][1] = __builtin_bit_cast(vec8, b);
@@ -348,7 +368,7 @@ struct RowState {
             for (int r = 0; r < NR; ++r) {
                 const int see = limit[r] - 64 * unit;
                 const unsigned long long seen = see <= 0 ? 0ull : see >= 64 ? ~0ull : (1ull << see) - 1;
-                nan[r] |= (unsigned long long)((k & seen) != 0) << e;
+                nan[r] |= (NanBits)((k & seen) != 0) << e;
             }
         }
     }
@@ -536,8 +556,12 @@ __global__ __launch_bounds__(256, 2) void cache_rows_kernel(CacheAttnParams p) {
                 if (!AHEAD) load_values(here, 0);
                 else if (more) load_keys(next);
                 else drop_keys();
+                if (boundary || (SMALL && __any(here.dead))) st.mask(s, key0, here.dead);
+                float top[NR];
+                st.peak(s, here.kf, top);
+                st.raise(top);
                 st.follow(here.top);
-                st.softmax(s, w, key0, here.kf, here.vs, here.dead, boundary || (SMALL && __any(here.dead)));
+                st.weights(s, w, here.kf, here.vs);
                 bool nan = false;
                 const auto part = [&](auto from) {
                     constexpr int D0 = decltype(from)::value;
@@ -631,6 +655,20 @@ __global__ __launch_bounds__(256, 2) void cache_rows_kernel(CacheAttnParams p) {
     }
 }
 
+// Order of a stretch of MFMAs products, READS operand reads from LDS and vector work: the first reads, then a read for every MFMAS / READS products with VALU vector
+// instructions behind each of them.  (Left to itself the compiler waits for every read where it is used and lets the two units take turns.)
+template <int MFMAS, int READS, int VALU, int AHEAD>
+__device__ __forceinline__ void mix() {
+    constexpr int PER = MFMAS / READS;
+    __builtin_amdgcn_sched_group_barrier(0x100, AHEAD, 0);
+#pragma unroll
+    for (int i = 0; i < READS; ++i) {
+        if (i + AHEAD < READS) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x008, PER, 0);
+        __builtin_amdgcn_sched_group_barrier(0x402, VALU, 0);
+    }
+}
+
 // query tiles of 16 rows per wave: two where O (16 NR W / 64 registers) leaves room for two waves per SIMD
 constexpr int tile_nr(int W) { return W <= 128 ? 2 : 1; }
 
@@ -662,28 +700,33 @@ __global__ __launch_bounds__(256, W > 128 ? 1 : 2) void cache_tile_kernel(CacheA
     const int see = rq.len - rq.n + last / p.group + 1;            // keys that the tile's last row sees
     const int units = see > 0 ? (see + 63) >> 6 : 0;
     const int u0 = (int)((long long)units * part / p.splits), u1 = (int)((long long)units * (part + 1) / p.splits);
-    const bool idle = row0 + 16 * NR * wave > last;                     // (a wave without rows still brings its share of the operands)
 
     const int tile_min = rq.len - rq.n + row0 / p.group + 1;        // keys that its first row sees
     if (threadIdx.x < 2) nan_found[threadIdx.x] = 0;
     __syncthreads();
 
-    // operands of a unit: wave w brings key tile w and the value columns of ND / 4 tiles
+    // Operands of a unit: wave w brings key tile w and the value columns of ND / 4 tiles.  The loop runs one unit ahead on the score side: while the
+    // matrix pipe forms S(u + 1), the vector unit forms the weights of u; while it adds V(u) P(u), the vector unit looks for the maxima of S(u + 1).  So
+    // the keys of u + 2 and the values of u + 1 are fetched in the middle of a round and spread into LDS at its end, two buffers each, one barrier.
     u32x4 kr[KPW], vr[VPW];
-    UnitAt<SMALL> here, next;
+    UnitAt<SMALL> here, next, after;
     const unsigned key_off = UnitAt<SMALL>::key_lane(W, lane), value_off = UnitAt<SMALL>::value_lane(p.shift, lane);
-    const auto load = [&](const UnitAt<SMALL>& a) {
+    const auto load_keys = [&](const UnitAt<SMALL>& a) {
 #pragma unroll
         for (int i = 0; i < KPW; ++i) kr[i] = *(const u32x4*)(a.k + (4 * wave * W + 64 * i) + key_off);
+    };
+    const auto load_values = [&](const UnitAt<SMALL>& a) {
 #pragma unroll
         for (int i = 0; i < VPW; ++i) vr[i] = *(const u32x4*)(a.v + ((16 * (wave * VPW + i)) << p.shift) + value_off);
     };
-    const auto spread = [&](const UnitAt<SMALL>& a, int u, int buf) {
+    const auto spread_keys = [&](int buf) {
 #pragma unroll
         for (int i = 0; i < KPW; ++i)
 #pragma unroll
             for (int c = 0; c < 2; ++c)
                 lds_k[buf][(wave * NC + 2 * i + c) * 64 + lane] = __builtin_bit_cast(u32x4, fragment<T>(kr[i][2 * c], kr[i][2 * c + 1]));
+    };
+    const auto spread_values = [&](const UnitAt<SMALL>& a, int u, int buf) {
         if (64 * u + 64 > rq.len || __any(a.blank)) {
             const int valid = a.blank ? 0 : rq.len - (64 * u + 16 * lg);
 #pragma unroll
@@ -704,35 +747,69 @@ __global__ __launch_bounds__(256, W > 128 ? 1 : 2) void cache_tile_kernel(CacheA
             for (int c = 0; c < 2; ++c)
                 lds_v[buf][((wave * VPW + i) * 2 + c) * 64 + lane] = __builtin_bit_cast(u32x4, fragment<T>(vr[i][2 * c], vr[i][2 * c + 1]));
     };
+    f32x4 s[2][NR][4];
+    const auto scores = [&](int buf, f32x4 (&to)[NR][4]) {
+        st.template scores<false>([&](int t, int c) { return __builtin_bit_cast(vec8, lds_k[buf][(t * NC + c) * 64 + lane]); }, to);
+    };
+    // what stands between a unit's scores and its weights
+    const auto prepare = [&](int u, const UnitAt<SMALL>& a, f32x4 (&x)[NR][4], float (&top)[NR]) {
+        if (64 * u + 64 > st.limit_min || __any(a.dead)) st.mask(x, 64 * u + 16 * lg, a.dead);
+        st.peak(x, a.kf, top);
+    };
     if (u0 < u1) {
         here.find(p, table, rq.len, u0, h, W, lane);
-        load(here);
-        spread(here, u0, 0);
+        load_keys(here);
+        load_values(here);
+        spread_keys(0);
+        spread_values(here, u0, 0);
+        next.find(p, table, rq.len, min(u0 + 1, u1 - 1), h, W, lane);
+        load_keys(next);
+        spread_keys(1);
     }
     __syncthreads();
-    for (int u = u0; u < u1; ++u) {
-        const int buf = (u - u0) & 1;
+    if (u0 < u1) {
+        float top[NR];
+        scores(0, s[0]);
+        prepare(u0, here, s[0], top);
+        st.raise(top);
+        st.follow(here.top);
+    }
+    __syncthreads();                                                // (unit u0's keys are read: round u0 fetches u0 + 2's over them)
+    const auto round = [&](int u, auto which) {
+        constexpr int A = decltype(which)::value, B = A ^ 1;        // buffers and scores of this unit and of the next
         const bool more = u + 1 < u1;
+        // (behind the end everything goes on with the last unit's operands, and is dropped: a branch round the fetches costs more registers than there are)
+        if (!SMALL) after.find(p, table, rq.len, min(u + 2, u1 - 1), h, W, lane);
+        vec8 w[NR][2];
+        __builtin_amdgcn_sched_barrier(0);
+        scores(B, s[B]);
+        st.weights(s[A], w, here.kf, here.vs);
+        mix<4 * NC * NR, 4 * NC, 7, 2>();
+        __builtin_amdgcn_sched_barrier(0);
+        if (SMALL) after.find(p, table, rq.len, min(u + 2, u1 - 1), h, W, lane);     // (addresses of every lane: formed where registers are free)
+        load_keys(after);                                           // (here, where the scores of u have left their registers)
+        load_values(next);
+        float top[NR];
+        if (64 * u + 128 > st.limit_min || __any(next.dead)) st.mask(s[B], 64 * u + 64 + 16 * lg, next.dead);
+        __builtin_amdgcn_sched_barrier(0);
+        st.template values<0, ND, false>([&](int d, int v) { return __builtin_bit_cast(vec8, lds_v[A][(d * 2 + v) * 64 + lane]); }, w);
+        st.peak(s[B], next.kf, top);
+        mix<2 * ND * NR, 2 * ND, 2, 2>();
+        __builtin_amdgcn_sched_barrier(0);
+        if (nan_found[A] == u + 1) st.note_nan((const unsigned long long*)nan_keys[A], u, lg);
         if (more) {
-            next.find(p, table, rq.len, u + 1, h, W, lane);
-            load(next);
+            st.raise(top);
+            st.follow(next.top);
         }
-        if (!here.none && !idle && 64 * u < st.limit_max) {
-            const int key0 = 64 * u + 16 * lg;
-            const bool boundary = 64 * u + 64 > st.limit_min;
-            f32x4 s[NR][4];
-            vec8 w[NR][2];
-            st.template scores<false>([&](int t, int c) { return __builtin_bit_cast(vec8, lds_k[buf][(t * NC + c) * 64 + lane]); }, s);
-            st.follow(here.top);
-            st.softmax(s, w, key0, here.kf, here.vs, here.dead, boundary || (SMALL && __any(here.dead)));
-            st.template values<0, ND, false>([&](int d, int v) { return __builtin_bit_cast(vec8, lds_v[buf][(d * 2 + v) * 64 + lane]); }, w);
-            if (nan_found[buf] == u + 1) st.note_nan((const unsigned long long*)nan_keys[buf], u, lg);
-        }
-        if (more) {
-            spread(next, u + 1, buf ^ 1);
-            here = next;
-        }
+        spread_values(next, u + 1, B);
+        spread_keys(A);
+        here = next;
+        next = after;
         __syncthreads();
+    };
+    for (int u = u0; u < u1; u += 2) {
+        round(u, std::integral_constant<int, 0>{});
+        if (u + 1 < u1) round(u + 1, std::integral_constant<int, 1>{});
     }
     st.finish();
     float sum[NR], top[NR];
