@@ -106,17 +106,24 @@ __device__ __forceinline__ unsigned take_nan(u32x4& v) {
     return bits;
 }
 
+// Tables, lengths and scales do not change while a kernel runs: read through the constant address space, uniform ones stay scalar loads behind a barrier (the
+// compiler takes a barrier for a change of all memory, and would wait for the codes in flight with every vector load in their place).
+template <typename V>
+__device__ __forceinline__ V constant(const V* p) {
+    return *(const __attribute__((address_space(4))) V*)(unsigned long long)p;
+}
+
 // ---- a request as every kernel here sees it: all indexes held inside what the caller's tensors have ----------------------------------------
 struct Request {
     int first, n, len, units;
 };
 __device__ __forceinline__ Request request_of(const CacheAttnParams& p, int b) {
     Request r;
-    const int a = min(max(p.cu_q[b], 0), p.T), e = min(max(p.cu_q[b + 1], a), p.T);
+    const int a = min(max(constant(p.cu_q + b), 0), p.T), e = min(max(constant(p.cu_q + b + 1), a), p.T);
     const long long room = (long long)p.width << p.shift;
     r.first = a;
     r.n = e - a;
-    r.len = max(p.seq_lens[b], 0);
+    r.len = max(constant(p.seq_lens + b), 0);
     r.len = r.len < room ? r.len : (int)room;
     r.units = max(1, (int)(((long long)r.len + 63) >> 6));
     return r;
@@ -416,7 +423,7 @@ struct RowState {
 
 // the block of a token index, -1 where the table has none that exists
 __device__ __forceinline__ int block_at(const CacheAttnParams& p, const int* table, int index) {
-    const int id = index < p.width ? table[index] : -1;
+    const int id = index < p.width ? constant(table + index) : -1;
     return (unsigned)id < (unsigned)p.num_blocks ? id : -1;
 }
 
@@ -441,8 +448,8 @@ struct UnitAt {
             const int in = first & (P - 1);
             k = p.k + blk * p.k_bs + (int64_t)(h * P + in) * W;
             v = p.v + blk * p.v_bs + (int64_t)h * P * W + in;
-            kf = factor(none ? 0.f : p.ks[blk * p.ks_bs + h] * p.scale_log2);
-            vs = none ? 0.f : p.vs[blk * p.vs_bs + h];
+            kf = factor(none ? 0.f : constant(p.ks + blk * p.ks_bs + h) * p.scale_log2);
+            vs = none ? 0.f : constant(p.vs + blk * p.vs_bs + h);
             blank = vs == 0.f;
             vs = factor(vs);
             top = vs;
@@ -455,8 +462,8 @@ struct UnitAt {
             const long long kb = kid < 0 ? 0 : kid, vb = vid < 0 ? 0 : vid;
             k = p.k + kb * p.k_bs + (int64_t)(h * P + (kk & (P - 1))) * W;
             v = p.v + vb * p.v_bs + (int64_t)h * P * W + (vk & (P - 1));
-            kf = factor(dead ? 0.f : p.ks[vb * p.ks_bs + h] * p.scale_log2);
-            vs = dead ? 0.f : p.vs[vb * p.vs_bs + h];
+            kf = factor(dead ? 0.f : constant(p.ks + vb * p.ks_bs + h) * p.scale_log2);
+            vs = dead ? 0.f : constant(p.vs + vb * p.vs_bs + h);
             blank = vs == 0.f;
             vs = factor(vs);
             top = rows_max(vs);
