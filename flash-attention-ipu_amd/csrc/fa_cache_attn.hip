@@ -791,7 +791,7 @@ __global__ __launch_bounds__(256, W > 128 ? 1 : 2) void cache_tile_kernel(CacheA
         __builtin_amdgcn_sched_barrier(0);
         scores(B, s[B]);
         st.weights(s[A], w, here.kf, here.vs);
-        mix<4 * NC * NR, 4 * NC, 7, 2>();
+        mix<4 * NC * NR, 4 * NC, 8, 2>();
         __builtin_amdgcn_sched_barrier(0);
         if (SMALL) after.find(p, table, rq.len, min(u + 2, u1 - 1), h, W, lane);     // (addresses of every lane: formed where registers are free)
         load_keys(after);                                           // (here, where the scores of u have left their registers)
@@ -801,7 +801,7 @@ __global__ __launch_bounds__(256, W > 128 ? 1 : 2) void cache_tile_kernel(CacheA
         __builtin_amdgcn_sched_barrier(0);
         st.template values<0, ND, false>([&](int d, int v) { return __builtin_bit_cast(vec8, lds_v[A][(d * 2 + v) * 64 + lane]); }, w);
         st.peak(s[B], next.kf, top);
-        mix<2 * ND * NR, 2 * ND, 2, 2>();
+        mix<2 * ND * NR, 2 * ND, 1, SMALL ? 2 : 4>();
         __builtin_amdgcn_sched_barrier(0);
         if (nan_found[A] == u + 1) st.note_nan((const unsigned long long*)nan_keys[A], u, lg);
         if (more) {
