@@ -479,6 +479,15 @@ struct UnitAt {
     }
 };
 
+// Codes are read once, so the row kernel asks for them past the caches' keeping (nontemporal: 108 instead of 123 us for 64 requests of 4600 tokens, 8 heads of
+// 128) - where a 128-byte line belongs to one wave's loads.  In blocks of 128 tokens a line of the values holds one column of TWO units, which two waves read:
+// it has to stay until the second one comes (142 instead of 126 us otherwise).
+template <bool ONCE>
+__device__ __forceinline__ u32x4 read_codes(const uint8_t* p) {
+    if constexpr (ONCE) return __builtin_nontemporal_load((const u32x4*)p);
+    else return *(const u32x4*)p;
+}
+
 // ---- row kernel ---------------------------------------------------------------------------------------------------------------------------
 // (whole: the line is made of row tiles, none of which is cut)
 __device__ __forceinline__ long long row_items(const CacheAttnParams& p, const Request& rq, int rows16) {
@@ -490,8 +499,10 @@ __device__ __forceinline__ long long range_of(const CacheAttnParams& p, long lon
     return per > p.min_units ? per : p.min_units;
 }
 
-template <typename T, int W, int NR, bool SMALL>
+// SHIFT: block size, 16 and 32 as one (4), 64 (6), 128 (7)
+template <typename T, int W, int NR, int SHIFT>
 __global__ __launch_bounds__(256, 2) void cache_rows_kernel(CacheAttnParams p) {
+    constexpr bool SMALL = SHIFT < 6;
     using State = RowState<T, W, NR>;
     constexpr int ND = State::ND, NK = W / 64, ROWS = 16 * NR;
     // the next unit's codes are fetched under this one's arithmetic where the registers hold them beside O; else a unit's value columns are
@@ -532,7 +543,7 @@ __global__ __launch_bounds__(256, 2) void cache_rows_kernel(CacheAttnParams p) {
 #pragma unroll
             for (int t = 0; t < 4; ++t)
 #pragma unroll
-                for (int i = 0; i < NK; ++i) kr[t][i] = *(const u32x4*)(a.k + (4 * t * W + 64 * i) + key_off);
+                for (int i = 0; i < NK; ++i) kr[t][i] = read_codes<true>(a.k + (4 * t * W + 64 * i) + key_off);
         };
         const auto drop_keys = [&]() {                     // (else the last unit's keys stay in registers for a round that never comes)
 #pragma unroll
@@ -543,7 +554,7 @@ __global__ __launch_bounds__(256, 2) void cache_rows_kernel(CacheAttnParams p) {
         const auto load_values = [&](const UnitAt<SMALL>& a, int d0) {
             const int step = fresh_scalar(16 << p.shift);
 #pragma unroll
-            for (int d = 0; d < VN; ++d) vr[d] = *(const u32x4*)(a.v + (d0 + d) * step + value_off);
+            for (int d = 0; d < VN; ++d) vr[d] = read_codes<SHIFT < 7>(a.v + (d0 + d) * step + value_off);
         };
         int u = u0 + wave;
         if (u < u1) {
@@ -910,13 +921,16 @@ __global__ __launch_bounds__(256) void cache_join_kernel(CacheAttnParams p, int 
     }
 }
 
+template <typename T, int W, int NR>
+const void* rows_kernel(int shift) {
+    return shift < 6 ? (const void*)cache_rows_kernel<T, W, NR, 4> : shift == 6 ? (const void*)cache_rows_kernel<T, W, NR, 6> : (const void*)cache_rows_kernel<T, W, NR, 7>;
+}
 template <typename T, int W>
 hipError_t launch_width(const CacheAttnParams& p, const CacheAttnPlan& plan, hipStream_t stream) {
     const bool small = p.shift < 6;
     const void* k;
     if (plan.tile) k = small ? (const void*)cache_tile_kernel<T, W, true> : (const void*)cache_tile_kernel<T, W, false>;
-    else if (W > 128 || plan.nr == 1) k = small ? (const void*)cache_rows_kernel<T, W, 1, true> : (const void*)cache_rows_kernel<T, W, 1, false>;
-    else k = small ? (const void*)cache_rows_kernel<T, W <= 128 ? W : 128, 2, true> : (const void*)cache_rows_kernel<T, W <= 128 ? W : 128, 2, false>;
+    else k = plan.nr == 1 || W > 128 ? rows_kernel<T, W, 1>(p.shift) : rows_kernel<T, (W <= 128 ? W : 128), 2>(p.shift);
     return launch1(k, dim3((unsigned)plan.grid), dim3(256), 0, stream, p);
 }
 template <typename T>
