@@ -38,8 +38,9 @@ struct RopeParams {
     int32_t pos64, L, D, R, interleaved, w_f32;
     float eps;
 };
-hipError_t launch_rope_fwd(const RopeParams& p, int dtype, bool vec, int heads_per_group, hipStream_t stream);
-hipError_t launch_rope_bwd(const RopeParams& p, int dtype, bool vec, int heads_per_group, hipStream_t stream);
+// vec: 16-byte accesses; stream_past: the data does not fit the last cache and is not kept there
+hipError_t launch_rope_fwd(const RopeParams& p, int dtype, bool vec, int heads_per_group, bool stream_past, hipStream_t stream);
+hipError_t launch_rope_bwd(const RopeParams& p, int dtype, bool vec, int heads_per_group, bool stream_past, hipStream_t stream);
 
 // ---- block tables, positions and slots of one step (fa_cache_update.hip) --------------------------------------------------------------
 struct TablesParams {

@@ -36,7 +36,7 @@ constexpr int kRopeFwdBlocks = 2048;          // forward: workgroups per side
 
 struct RopeCall {
     fa::RopeParams p;
-    bool vec;
+    bool vec, stream_past;
     int hc, es;
 };
 
@@ -75,13 +75,16 @@ int rope_common(RopeCall* c, const void* q_weight, const void* k_weight, int32_t
     return FA_OK;
 }
 
-// heads per lane group, items and workgroups of both sides.  Several heads per lane group fetch cosines, sines and position once and keep more loads
-// in flight, but a launch of few rows needs its lanes: measured at [T, 32 + 8, 128] bf16, see fa_rope.hip's table
+// Heads per lane group, items and workgroups of both sides.  Two heads per lane group fetch cosines, sines and position once and keep more loads in
+// flight ([4, 4096, 32 + 8, 128] bf16: 60.9 us, four heads 62.7), but a launch of few rows needs its lanes ([64, 32 + 8, 128]: 4.1 us with one).  What moves more
+// than the 256 MB of the last cache is read and written past it: forward 62.7 -> 60.9, backward 98.6 -> 91.8 us there; 50 MB that the next kernel
+// finds in the cache lose by it (forward 11.9 -> 13.7 us).
 void rope_shape(RopeCall* c, int64_t B, bool backward) {
     fa::RopeParams& p = c->p;
-    const int lpr = c->vec ? p.D / 16 : 64, many = backward ? 2 : 4;
+    const int lpr = c->vec ? p.D * c->es / 32 : 64;
     const int64_t tokens = B * p.L, rows = tokens * (p.side[0].heads + p.side[1].heads);
-    c->hc = c->vec && rows * lpr / 64 >= 8192 ? many : 1;
+    c->hc = c->vec && rows * lpr / 64 >= 8192 ? 2 : 1;
+    c->stream_past = rows * p.D * c->es * (backward ? 3 : 2) > (256ll << 20);
     for (fa::RopeSide& s : p.side) {
         s.chunks = (int32_t)up(s.heads, c->hc);
         s.items = (int32_t)(tokens * s.chunks);
@@ -188,7 +191,7 @@ int fa_qk_norm_rope_fwd(const void* q, const void* k, void* q_out, void* k_out, 
         if (!aligned(in[i], c.es) || !aligned(out[i], c.es)) return fail(FA_ERR_MISALIGNED, "operands must be aligned to their element size");
     }
     rope_shape(&c, B, false);
-    return launched(fa::launch_rope_fwd(c.p, dtype, c.vec, c.hc, (hipStream_t)stream));
+    return launched(fa::launch_rope_fwd(c.p, dtype, c.vec, c.hc, c.stream_past, (hipStream_t)stream));
 }
 
 int64_t fa_qk_norm_rope_workspace(int64_t B, int64_t L, int64_t heads, int64_t heads_kv, int64_t D) {
@@ -225,7 +228,7 @@ int fa_qk_norm_rope_bwd(const void* q, const void* k, const void* dq_out, const 
         if (!aligned(in[i], c.es) || !aligned(din[i], c.es) || !aligned(out[i], c.es)) return fail(FA_ERR_MISALIGNED, "operands must be aligned to their element size");
     }
     rope_shape(&c, B, true);
-    return launched(fa::launch_rope_bwd(c.p, dtype, c.vec, c.hc, (hipStream_t)stream));
+    return launched(fa::launch_rope_bwd(c.p, dtype, c.vec, c.hc, c.stream_past, (hipStream_t)stream));
 }
 
 int fa_cache_tables(const int32_t* seq_lens, const int32_t* new_lens, int32_t* block_tables, int64_t table_stride, int64_t max_blocks, int32_t* free_blocks,

@@ -5,8 +5,8 @@
 //   backward: g = turn back(d out);  dw = sum over rows g x r;  t = g w;  dx = r (t - x r mean(t x r)).
 //
 // Bound: memory.  Forward reads and writes every value once; backward reads x and d out once and writes dx.  A row is held in the
-// registers of D / 16 lanes, eight columns of each half of the pairs per lane (two 16-byte loads of 16-bit values), so that both members of a
-// pair are in one lane and the mean costs log2(D / 16) lane exchanges.  A lane group takes HC heads of one token: cosines, sines and
+// registers of a few lanes (8 for 128 columns of 16 bits), a run of 16 bytes of each half of the pairs per lane, so that both members of a
+// pair are in one lane and the mean costs a lane exchange per halving.  A lane group takes HC heads of one token: cosines, sines and
 // the position are fetched once for them and HC rows' loads are in flight together.  Sums, statistics and angles are 32-bit.
 // dw has no atomics: a workgroup keeps its sum in registers over a fixed set of rows, writes one [D] row, and a second kernel adds the rows in order.
 // A position below 0 marks a row of padding: its outputs and gradients are zeros.  A position behind the table gives NaN.
@@ -18,20 +18,27 @@
 namespace fa {
 namespace {
 
-template <typename T> struct Vec8 { typedef T type __attribute__((ext_vector_type(8))); };
+// runs of E columns that a lane holds: 16 bytes, so that every access of a wave is whole lines
+template <typename T> constexpr int kRun = 16 / (int)sizeof(T);
+template <typename T, int E> struct Vec { typedef T type __attribute__((ext_vector_type(E))); };
 
-template <typename T>
-__device__ __forceinline__ void load8(const T* p, float (&f)[8]) {
-    const typename Vec8<T>::type v = *(const typename Vec8<T>::type*)p;
+template <bool STREAM, typename T, int E>
+__device__ __forceinline__ void load_run(const T* p, float (&f)[E]) {
+    using V = typename Vec<T, E>::type;
+    V v;
+    if constexpr (STREAM) v = __builtin_nontemporal_load((const V*)p);
+    else v = *(const V*)p;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) f[i] = (float)v[i];
+    for (int i = 0; i < E; ++i) f[i] = (float)v[i];
 }
-template <typename T>
-__device__ __forceinline__ void store8(T* p, const float (&f)[8]) {
-    typename Vec8<T>::type v;
+template <bool STREAM, typename T, int E>
+__device__ __forceinline__ void store_run(T* p, const float (&f)[E]) {
+    using V = typename Vec<T, E>::type;
+    V v;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = (T)f[i];
-    *(typename Vec8<T>::type*)p = v;
+    for (int i = 0; i < E; ++i) v[i] = (T)f[i];
+    if constexpr (STREAM) __builtin_nontemporal_store(v, (V*)p);
+    else *(V*)p = v;
 }
 
 template <int CTRL>
@@ -60,14 +67,14 @@ __device__ __forceinline__ int64_t row_of(const RopeParams& p, int b, int l) {
     return pos < 0 ? -1 : pos < p.table_rows ? pos : p.table_rows;
 }
 
-// eight weights of columns c .. c + 7 (16-byte aligned; ones without weights)
-template <typename T>
-__device__ __forceinline__ void weights8(const RopeParams& p, const void* w, int c, float (&f)[8]) {
+// the weights of columns c .. c + E - 1 (16-byte aligned; ones without weights)
+template <typename T, int E>
+__device__ __forceinline__ void weight_run(const RopeParams& p, const void* w, int c, float (&f)[E]) {
     if (w == nullptr) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) f[i] = 1.0f;
-    } else if (p.w_f32) load8((const float*)w + c, f);
-    else load8((const T*)w + c, f);
+        for (int i = 0; i < E; ++i) f[i] = 1.0f;
+    } else if (p.w_f32) load_run<false>((const float*)w + c, f);
+    else load_run<false>((const T*)w + c, f);
 }
 template <typename T>
 __device__ __forceinline__ float weight_at(const RopeParams& p, const void* w, int i) {
@@ -89,45 +96,45 @@ __device__ __forceinline__ void item_of(const RopeSide& s, int L, unsigned item,
     }
 }
 
-// turn (sign = 1) or turn back (sign = -1) the pairs that a lane holds: f0, f1 are its two runs of eight columns
-template <bool INTER>
-__device__ __forceinline__ void turn(float (&f0)[8], float (&f1)[8], const float (&c)[8], const float (&s)[8], float sign) {
+// turn (sign = 1) or turn back (sign = -1) the pairs that a lane holds: f0, f1 are its two runs of columns
+template <bool INTER, int E>
+__device__ __forceinline__ void turn(float (&f0)[E], float (&f1)[E], const float (&c)[E], const float (&s)[E], float sign) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        float& a = INTER ? (i < 4 ? f0[2 * i] : f1[2 * i - 8]) : f0[i];
-        float& b = INTER ? (i < 4 ? f0[2 * i + 1] : f1[2 * i - 7]) : f1[i];
+    for (int i = 0; i < E; ++i) {
+        float& a = INTER ? (i < E / 2 ? f0[2 * i] : f1[2 * i - E]) : f0[i];
+        float& b = INTER ? (i < E / 2 ? f0[2 * i + 1] : f1[2 * i + 1 - E]) : f1[i];
         const float sn = s[i] * sign, a0 = a, b0 = b;
         a = a0 * c[i] - b0 * sn;
         b = a0 * sn + b0 * c[i];
     }
 }
 
-// D = 16 LPR, 16-byte rows, R a multiple of 16
-template <typename T, int LPR, bool INTER, int HC, bool BWD>
+// D = 2 E LPR, 16-byte rows, R a multiple of 16.  STREAM: the launch moves more than the last cache holds, so that nothing is kept in it (rope_shape)
+template <typename T, int LPR, bool INTER, int HC, bool BWD, bool STREAM>
 __global__ __launch_bounds__(256) void rope_vec_kernel(RopeParams p) {
     const int which = (int)blockIdx.x >= p.side[0].blocks;
     const RopeSide& s = p.side[which];
     const int block = which ? (int)blockIdx.x - p.side[0].blocks : (int)blockIdx.x;
-    constexpr int D = 16 * LPR, GROUPS = 256 / LPR;
+    constexpr int E = kRun<T>, D = 2 * E * LPR, GROUPS = 256 / LPR;
     const int j = (int)threadIdx.x % LPR, group = (int)threadIdx.x / LPR;
-    const int R = p.R, rot = R / 16;
+    const int R = p.R, rot = R / (2 * E);
     const bool rotated = j < rot;
-    int c0, c1;             // the lane's two runs of eight columns
+    int c0, c1;             // the lane's two runs of columns
     if (INTER) {
-        c0 = 16 * j;
-        c1 = c0 + 8;
+        c0 = 2 * E * j;
+        c1 = c0 + E;
     } else if (rotated) {
-        c0 = 8 * j;
-        c1 = R / 2 + 8 * j;
+        c0 = E * j;
+        c1 = R / 2 + E * j;
     } else {
-        c0 = R + 8 * (j - rot);
-        c1 = R + (D - R) / 2 + 8 * (j - rot);
+        c0 = R + E * (j - rot);
+        c1 = R + (D - R) / 2 + E * (j - rot);
     }
-    float w0[8], w1[8], dw0[8], dw1[8];
-    weights8<T>(p, s.w, c0, w0);
-    weights8<T>(p, s.w, c1, w1);
+    float w0[E], w1[E], dw0[E], dw1[E];
+    weight_run<T>(p, s.w, c0, w0);
+    weight_run<T>(p, s.w, c1, w1);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) dw0[i] = dw1[i] = 0.f;
+    for (int i = 0; i < E; ++i) dw0[i] = dw1[i] = 0.f;
     const T* x = (const T*)s.x;
     const T* dy = (const T*)s.dy;
     T* y = (T*)s.y;
@@ -135,32 +142,32 @@ __global__ __launch_bounds__(256) void rope_vec_kernel(RopeParams p) {
         int b, l, c;
         item_of(s, p.L, (unsigned)item, b, l, c);
         const int64_t pos = row_of(p, b, l);
-        float f0[HC][8], f1[HC][8], g0[HC][8], g1[HC][8], cs[8], sn[8];
+        float f0[HC][E], f1[HC][E], g0[HC][E], g1[HC][E], cs[E], sn[E];
 #pragma unroll
         for (int h = 0; h < HC; ++h) {
             const int head = c + h * s.chunks;
             if (head < s.heads) {
                 const T* row = x + (int64_t)b * s.x_sb + (int64_t)head * s.x_sh + (int64_t)l * s.x_sl;
-                load8(row + c0, f0[h]);
-                load8(row + c1, f1[h]);
+                load_run<STREAM>(row + c0, f0[h]);
+                load_run<STREAM>(row + c1, f1[h]);
                 if constexpr (BWD) {
                     const T* drow = dy + (int64_t)b * s.dy_sb + (int64_t)head * s.dy_sh + (int64_t)l * s.dy_sl;
-                    load8(drow + c0, g0[h]);
-                    load8(drow + c1, g1[h]);
+                    load_run<STREAM>(drow + c0, g0[h]);
+                    load_run<STREAM>(drow + c1, g1[h]);
                 }
             }
         }
 #pragma unroll
-        for (int i = 0; i < 8; ++i) { cs[i] = 1.f; sn[i] = 0.f; }
+        for (int i = 0; i < E; ++i) { cs[i] = 1.f; sn[i] = 0.f; }
         const bool pad = pos < 0;
         if (rotated && pos >= 0 && pos < p.table_rows) {
-            const float* t = p.table + pos * R + 8 * j;
-            load8(t, cs);
-            load8(t + R / 2, sn);
+            const float* t = p.table + pos * R + E * j;
+            load_run<false>(t, cs);
+            load_run<false>(t + R / 2, sn);
         }
         if (pos == p.table_rows) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) cs[i] = sn[i] = __builtin_nanf("");
+            for (int i = 0; i < E; ++i) cs[i] = sn[i] = __builtin_nanf("");
         }
 #pragma unroll
         for (int h = 0; h < HC; ++h) {
@@ -168,20 +175,20 @@ __global__ __launch_bounds__(256) void rope_vec_kernel(RopeParams p) {
             if (head >= s.heads) continue;
             float sq = 0.f;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) sq += f0[h][i] * f0[h][i];
+            for (int i = 0; i < E; ++i) sq += f0[h][i] * f0[h][i];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) sq += f1[h][i] * f1[h][i];
+            for (int i = 0; i < E; ++i) sq += f1[h][i] * f1[h][i];
             const float r = rsqrtf(group_sum<LPR>(sq) * (1.0f / D) + p.eps);
-            float o0[8], o1[8];
+            float o0[E], o1[E];
             if constexpr (!BWD) {
 #pragma unroll
-                for (int i = 0; i < 8; ++i) { o0[i] = f0[h][i] * r * w0[i]; o1[i] = f1[h][i] * r * w1[i]; }
+                for (int i = 0; i < E; ++i) { o0[i] = f0[h][i] * r * w0[i]; o1[i] = f1[h][i] * r * w1[i]; }
                 turn<INTER>(o0, o1, cs, sn, 1.f);
             } else {
                 turn<INTER>(g0[h], g1[h], cs, sn, -1.f);
                 float dot = 0.f;
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
+                for (int i = 0; i < E; ++i) {
                     const float h0 = f0[h][i] * r, h1 = f1[h][i] * r;
                     if (!pad) { dw0[i] += g0[h][i] * h0; dw1[i] += g1[h][i] * h1; }
                     o0[i] = g0[h][i] * w0[i];
@@ -192,15 +199,15 @@ __global__ __launch_bounds__(256) void rope_vec_kernel(RopeParams p) {
                 }
                 const float m = group_sum<LPR>(dot) * (1.0f / D);
 #pragma unroll
-                for (int i = 0; i < 8; ++i) { o0[i] = r * (o0[i] - f0[h][i] * m); o1[i] = r * (o1[i] - f1[h][i] * m); }
+                for (int i = 0; i < E; ++i) { o0[i] = r * (o0[i] - f0[h][i] * m); o1[i] = r * (o1[i] - f1[h][i] * m); }
             }
             if (pad) {
 #pragma unroll
-                for (int i = 0; i < 8; ++i) o0[i] = o1[i] = 0.f;
+                for (int i = 0; i < E; ++i) o0[i] = o1[i] = 0.f;
             }
             T* row = y + (int64_t)b * s.y_sb + (int64_t)head * s.y_sh + (int64_t)l * s.y_sl;
-            store8(row + c0, o0);
-            store8(row + c1, o1);
+            store_run<STREAM>(row + c0, o0);
+            store_run<STREAM>(row + c1, o1);
         }
     }
     if constexpr (BWD) {
@@ -209,7 +216,7 @@ __global__ __launch_bounds__(256) void rope_vec_kernel(RopeParams p) {
         __shared__ float part[4][D];
         const int lane = (int)threadIdx.x & 63, wave = (int)threadIdx.x >> 6;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
+        for (int i = 0; i < E; ++i) {
 #pragma unroll
             for (int d = LPR; d < 64; d *= 2) {
                 dw0[i] += __shfl_xor(dw0[i], d);
@@ -218,7 +225,7 @@ __global__ __launch_bounds__(256) void rope_vec_kernel(RopeParams p) {
         }
         if (lane < LPR) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) { part[wave][c0 + i] = dw0[i]; part[wave][c1 + i] = dw1[i]; }
+            for (int i = 0; i < E; ++i) { part[wave][c0 + i] = dw0[i]; part[wave][c1 + i] = dw1[i]; }
         }
         __syncthreads();
         for (int d = (int)threadIdx.x; d < D; d += 256) s.dw_part[(int64_t)block * D + d] = part[0][d] + part[1][d] + part[2][d] + part[3][d];
@@ -346,19 +353,20 @@ __global__ __launch_bounds__(1024) void rope_dw_kernel(RopeParams p) {
 }
 
 template <typename T, int LPR, bool INTER, bool BWD>
-const void* vec_kernel(int hc) {
-    constexpr int MANY = BWD ? 2 : 4;
-    return hc == 1 ? (const void*)rope_vec_kernel<T, LPR, INTER, 1, BWD> : (const void*)rope_vec_kernel<T, LPR, INTER, MANY, BWD>;
+const void* vec_kernel(int hc, bool stream) {
+    return hc == 1 ? (const void*)rope_vec_kernel<T, LPR, INTER, 1, BWD, false>
+         : stream ? (const void*)rope_vec_kernel<T, LPR, INTER, 2, BWD, true> : (const void*)rope_vec_kernel<T, LPR, INTER, 2, BWD, false>;
 }
 template <typename T, bool INTER, bool BWD>
-const void* vec_kernel(int D, int hc) {
-    return D == 32 ? vec_kernel<T, 2, INTER, BWD>(hc) : D == 64 ? vec_kernel<T, 4, INTER, BWD>(hc)
-         : D == 128 ? vec_kernel<T, 8, INTER, BWD>(hc) : vec_kernel<T, 16, INTER, BWD>(hc);
+const void* vec_kernel(int D, int hc, bool stream) {
+    constexpr int L = 16 / kRun<T>;          // lanes of 32 columns
+    return D == 32 ? vec_kernel<T, L, INTER, BWD>(hc, stream) : D == 64 ? vec_kernel<T, 2 * L, INTER, BWD>(hc, stream)
+         : D == 128 ? vec_kernel<T, 4 * L, INTER, BWD>(hc, stream) : vec_kernel<T, 8 * L, INTER, BWD>(hc, stream);
 }
 template <typename T, bool BWD>
-hipError_t launch_rope(const RopeParams& p, bool vec, int hc, hipStream_t stream) {
+hipError_t launch_rope(const RopeParams& p, bool vec, int hc, bool nt, hipStream_t stream) {
     const dim3 grid((unsigned)(p.side[0].blocks + p.side[1].blocks));
-    const void* k = !vec ? (const void*)rope_any_kernel<T, BWD> : p.interleaved ? vec_kernel<T, true, BWD>(p.D, hc) : vec_kernel<T, false, BWD>(p.D, hc);
+    const void* k = !vec ? (const void*)rope_any_kernel<T, BWD> : p.interleaved ? vec_kernel<T, true, BWD>(p.D, hc, nt) : vec_kernel<T, false, BWD>(p.D, hc, nt);
     hipError_t e = launch1(k, grid, dim3(256), 0, stream, p);
     if (e == hipSuccess && BWD && (p.side[0].dw || p.side[1].dw))
         e = launch1((const void*)rope_dw_kernel<T>, dim3((unsigned)(p.D + 63) / 64, 2), dim3(1024), 0, stream, p);
@@ -367,13 +375,13 @@ hipError_t launch_rope(const RopeParams& p, bool vec, int hc, hipStream_t stream
 
 }  // namespace
 
-hipError_t launch_rope_fwd(const RopeParams& p, int dtype, bool vec, int hc, hipStream_t stream) {
-    return dtype == 0 ? launch_rope<_Float16, false>(p, vec, hc, stream) : dtype == 1 ? launch_rope<__bf16, false>(p, vec, hc, stream)
-                                                                                      : launch_rope<float, false>(p, vec, hc, stream);
+hipError_t launch_rope_fwd(const RopeParams& p, int dtype, bool vec, int hc, bool nt, hipStream_t stream) {
+    return dtype == 0 ? launch_rope<_Float16, false>(p, vec, hc, nt, stream) : dtype == 1 ? launch_rope<__bf16, false>(p, vec, hc, nt, stream)
+                                                                                      : launch_rope<float, false>(p, vec, hc, nt, stream);
 }
-hipError_t launch_rope_bwd(const RopeParams& p, int dtype, bool vec, int hc, hipStream_t stream) {
-    return dtype == 0 ? launch_rope<_Float16, true>(p, vec, hc, stream) : dtype == 1 ? launch_rope<__bf16, true>(p, vec, hc, stream)
-                                                                                     : launch_rope<float, true>(p, vec, hc, stream);
+hipError_t launch_rope_bwd(const RopeParams& p, int dtype, bool vec, int hc, bool nt, hipStream_t stream) {
+    return dtype == 0 ? launch_rope<_Float16, true>(p, vec, hc, nt, stream) : dtype == 1 ? launch_rope<__bf16, true>(p, vec, hc, nt, stream)
+                                                                                     : launch_rope<float, true>(p, vec, hc, nt, stream);
 }
 
 }  // namespace fa

@@ -17,8 +17,8 @@ static bool g_vec;
 static int g_hc;
 
 namespace fa {
-hipError_t launch_rope_fwd(const RopeParams& p, int, bool vec, int hc, hipStream_t) { ++g_launches; g_rope = p; g_vec = vec; g_hc = hc; return hipSuccess; }
-hipError_t launch_rope_bwd(const RopeParams& p, int, bool vec, int hc, hipStream_t) { ++g_launches; g_rope = p; g_vec = vec; g_hc = hc; return hipSuccess; }
+hipError_t launch_rope_fwd(const RopeParams& p, int, bool vec, int hc, bool, hipStream_t) { ++g_launches; g_rope = p; g_vec = vec; g_hc = hc; return hipSuccess; }
+hipError_t launch_rope_bwd(const RopeParams& p, int, bool vec, int hc, bool, hipStream_t) { ++g_launches; g_rope = p; g_vec = vec; g_hc = hc; return hipSuccess; }
 hipError_t launch_cache_tables(const TablesParams&, hipStream_t) { ++g_launches; return hipSuccess; }
 hipError_t launch_cache_append(const AppendParams& p, int, hipStream_t) { ++g_launches; g_append = p; return hipSuccess; }
 hipError_t launch_cache_attn(const CacheAttnParams& p, const CacheAttnPlan& plan, int, hipStream_t) { ++g_launches; g_attn = p; g_plan = plan; return hipSuccess; }
@@ -73,7 +73,7 @@ int main() {
             const fa::RopeSide& s = g_rope.side[i];
             CHECK((int64_t)s.chunks * g_hc >= s.heads && (int64_t)(s.chunks - 1) * g_hc < s.heads && s.items == B * L * s.chunks && s.blocks >= 1);
             if (bwd) CHECK((char*)(s.dw_part + (int64_t)s.blocks * D) <= buf + fa_qk_norm_rope_workspace(B, L, H, 2, D));
-            else CHECK(s.blocks >= 2048 /* the kernels stride over more */ || (int64_t)s.blocks * 256 >= (int64_t)s.items * (g_vec ? D / 16 : 64));
+            else CHECK(s.blocks >= 2048 /* the kernels stride over more */ || (int64_t)s.blocks * 256 >= (int64_t)s.items * (g_vec ? D * 2 / 32 : 64));
         }
     }
     // ---- tables
