@@ -16,32 +16,46 @@ namespace {
 // Bound: latency - a few kilobytes through one workgroup, three scans.  Sums saturate at 2^31 - 1 (which stays associative, so that the
 // scan order does not matter) where lengths add up to more.
 constexpr int kScanThreads = 1024;
+constexpr int kBatch = 4;       // entries per thread whose loads are in flight together
 
 __device__ __forceinline__ int sat_add(int a, int b) {
     const unsigned s = (unsigned)a + (unsigned)b;
     return s > 0x7fffffffu ? 0x7fffffff : (int)s;
 }
-// exclusive scan over the workgroup with saturation; `total` is every thread's
-__device__ __forceinline__ int block_scan(int x, int* waves, int& total) {
+// inclusive scan with saturation over a wave, through the data-parallel moves: inside rows of 16 lanes, then the rows' last lanes onto the rows behind them
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int scan_step(int x) {
+    return sat_add(x, __builtin_amdgcn_update_dpp(0, x, CTRL, ROWS, 0xf, false));
+}
+__device__ __forceinline__ int wave_scan(int x) {
+    x = scan_step<0x111, 0xf>(x);      // row_shr 1, 2, 4, 8
+    x = scan_step<0x112, 0xf>(x);
+    x = scan_step<0x114, 0xf>(x);
+    x = scan_step<0x118, 0xf>(x);
+    x = scan_step<0x142, 0xa>(x);      // row_bcast 15 onto rows 1 and 3
+    return scan_step<0x143, 0xc>(x);   // row_bcast 31 onto rows 2 and 3
+}
+// exclusive scans of N numbers over the workgroup; totals are every thread's
+template <int N>
+__device__ __forceinline__ void block_scan(const int (&x)[N], int (&before)[N], int (&total)[N], int (*waves)[kScanThreads / 64]) {
     const int lane = (int)threadIdx.x & 63, wave = (int)threadIdx.x >> 6;
-    int incl = x;
 #pragma unroll
-    for (int d = 1; d < 64; d *= 2) {
-        const int y = __shfl_up(incl, d);
-        if (lane >= d) incl = sat_add(incl, y);
-    }
-    if (lane == 63) waves[wave] = incl;
-    __syncthreads();
-    int before = 0;
-    total = 0;
-#pragma unroll
-    for (int w = 0; w < kScanThreads / 64; ++w) {
-        if (w == wave) before = total;
-        total = sat_add(total, waves[w]);
+    for (int n = 0; n < N; ++n) {
+        const int incl = wave_scan(x[n]);
+        if (lane == 63) waves[n][wave] = incl;
+        const int prev = __builtin_amdgcn_update_dpp(0, incl, 0x138, 0xf, 0xf, false);      // wave_shr 1
+        before[n] = lane ? prev : 0;
     }
     __syncthreads();
-    const int prev = __shfl_up(incl, 1);
-    return sat_add(before, lane ? prev : 0);
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+        // the waves' sums, scanned by every wave for itself
+        const int sums = wave_scan(lane < kScanThreads / 64 ? waves[n][lane] : 0);
+        total[n] = __builtin_amdgcn_readlane(sums, kScanThreads / 64 - 1);
+        const int ahead = __builtin_amdgcn_readlane(sums, wave ? __builtin_amdgcn_readfirstlane(wave) - 1 : 0);
+        before[n] = sat_add(wave ? ahead : 0, before[n]);
+    }
+    __syncthreads();
 }
 // largest i in [0, n) with first[i] <= x; first is ascending, first[0] <= x
 __device__ __forceinline__ int find(const int* first, int n, int x) {
@@ -67,7 +81,7 @@ __device__ __forceinline__ void place(const TablesParams& p, int t, int b, int s
 }
 
 __global__ __launch_bounds__(kScanThreads) void cache_tables_kernel(TablesParams p) {
-    __shared__ int waves[kScanThreads / 64], first[kScanThreads], start[kScanThreads], have_s[kScanThreads];
+    __shared__ int waves[1][kScanThreads / 64], first[kScanThreads], start[kScanThreads], have_s[kScanThreads], served_to;
     const int tid = (int)threadIdx.x;
     int free = *p.free_in;
     free = free < 0 ? 0 : free > p.pool_size ? p.pool_size : free;
@@ -75,51 +89,79 @@ __global__ __launch_bounds__(kScanThreads) void cache_tables_kernel(TablesParams
     for (int base = 0; base < p.B; base += kScanThreads) {
         const int b = base + tid;
         const bool ends = b < p.B && p.new_lens[b] < 0;
+        if (!__syncthreads_or(ends)) continue;
         const int held = ends ? max(p.seq_in[b], 0) : 0;
-        const int back = ends ? min(blocks_of(held, p.shift), p.width) : 0;
-        int total;
-        const int at = block_scan(back, waves, total);
-        if (total > 0) {                       // (uniform)
-            first[tid] = at;
-            __syncthreads();
-            for (int i = tid; i < total; i += kScanThreads) {
-                const int r = find(first, kScanThreads, i), to = sat_add(free, i);
-                if (to < p.pool_size) p.pool[to] = p.tables[(int64_t)(base + r) * p.table_stride + (i - first[r])];
+        const int back[1] = {ends ? min(blocks_of(held, p.shift), p.width) : 0};
+        int at[1], total[1];
+        block_scan<1>(back, at, total, waves);
+        first[tid] = at[0];
+        __syncthreads();
+        const int bound = min(total[0], p.pool_size - free);
+        for (int i0 = tid; i0 < bound; i0 += kBatch * kScanThreads) {
+            int id[kBatch];
+#pragma unroll
+            for (int k = 0; k < kBatch; ++k) {
+                const int i = i0 + k * kScanThreads;
+                if (i >= bound) continue;
+                const int r = find(first, min(p.B - base, kScanThreads), i);
+                id[k] = p.tables[(int64_t)(base + r) * p.table_stride + (i - first[r])];
             }
-            __syncthreads();
+#pragma unroll
+            for (int k = 0; k < kBatch; ++k)
+                if (i0 + k * kScanThreads < bound) p.pool[free + i0 + k * kScanThreads] = id[k];
         }
-        free = min(sat_add(free, total), p.pool_size);
+        __syncthreads();
+        free = min(sat_add(free, total[0]), p.pool_size);
     }
     // 2. and 3.
     int tokens = 0, needed = 0, taken = 0;     // running sums over the chunks of requests
     for (int base = 0; base < p.B; base += kScanThreads) {
-        const int b = base + tid;
+        const int b = base + tid, here = min(p.B - base, kScanThreads);
         const bool in = b < p.B;
         const int n = in ? p.new_lens[b] : 0, count = max(n, 0), held = in ? max(p.seq_in[b], 0) : 0;
-        int total;
-        const int my_start = sat_add(tokens, block_scan(count, waves, total)), my_end = sat_add(my_start, count);
-        tokens = sat_add(tokens, total);
         const int have = blocks_of(held, p.shift);
         const int64_t after = ((int64_t)held + count + (1 << p.shift) - 1) >> p.shift;
-        const bool fits = in && n >= 0 && after <= p.width && my_end <= p.T;
-        const int need = fits ? (int)after - have : 0;
-        const int before = sat_add(needed, block_scan(need, waves, total));
-        needed = sat_add(needed, total);
+        int my_start, my_end, need, before;
+        bool fits = in && n >= 0 && after <= p.width;
+        {
+            const int x[1] = {count};
+            int y[1], total[1];
+            block_scan<1>(x, y, total, waves);
+            my_start = sat_add(tokens, y[0]);
+            my_end = sat_add(my_start, count);
+            tokens = sat_add(tokens, total[0]);
+            fits = fits && my_end <= p.T;
+        }
+        {
+            need = fits ? (int)after - have : 0;
+            const int x[1] = {need};
+            int y[1], total[1];
+            if (tid == 0) served_to = taken;
+            block_scan<1>(x, y, total, waves);
+            before = sat_add(needed, y[0]);
+            needed = sat_add(needed, total[0]);
+        }
+        // (needs add up: once one is not met, none behind it is, so that a served request's blocks begin at `before`)
         const bool served = fits && (need == 0 || sat_add(before, need) <= free);
         const int granted = served ? count : 0;
-        const int add = served ? need : 0;
-        const int my_first = sat_add(taken, block_scan(add, waves, total));
-        if (total > 0) {                       // (uniform)
-            first[tid] = my_first;
-            have_s[tid] = have;
-            __syncthreads();
-            for (int i = tid; i < total; i += kScanThreads) {
-                const int k = taken + i, r = find(first, kScanThreads, k);
-                p.tables[(int64_t)(base + r) * p.table_stride + have_s[r] + (k - first[r])] = p.pool[free - 1 - k];
+        if (served && need > 0) atomicMax(&served_to, before + need);
+        first[tid] = before;
+        have_s[tid] = have;
+        __syncthreads();
+        const int upto = served_to;
+        for (int k0 = taken + tid; k0 < upto; k0 += kBatch * kScanThreads) {
+            int id[kBatch];
+#pragma unroll
+            for (int i = 0; i < kBatch; ++i) id[i] = k0 + i * kScanThreads < upto ? p.pool[free - 1 - k0 - i * kScanThreads] : 0;
+#pragma unroll
+            for (int i = 0; i < kBatch; ++i) {
+                const int k = k0 + i * kScanThreads;
+                if (k >= upto) continue;
+                const int r = find(first, here, k);
+                p.tables[(int64_t)(base + r) * p.table_stride + have_s[r] + (k - first[r])] = id[i];
             }
-            __syncthreads();
         }
-        taken += total;
+        taken = upto;
         const int held_after = n < 0 ? 0 : held + granted;
         if (in) {
             p.seq_out[b] = held_after;
@@ -127,6 +169,7 @@ __global__ __launch_bounds__(kScanThreads) void cache_tables_kernel(TablesParams
             p.cu_new[b] = my_start;
             if (b == p.B - 1) p.cu_new[p.B] = my_end;
         }
+        __syncthreads();
         if (p.fused) {
             // the tokens of this chunk of requests; first / start / have_s serve as request starts, grants and lengths
             first[tid] = my_start;
@@ -135,7 +178,7 @@ __global__ __launch_bounds__(kScanThreads) void cache_tables_kernel(TablesParams
             __syncthreads();
             const int from = base == 0 ? 0 : first[0], to = min(tokens, p.T);
             for (int t = from + tid; t < to; t += kScanThreads) {
-                const int r = find(first, min(p.B - base, kScanThreads), t);
+                const int r = find(first, here, t);
                 place(p, t, base + r, first[r], start[r], have_s[r]);
             }
             __syncthreads();
