@@ -162,7 +162,8 @@ int attn_plan(int64_t B, int64_t T, int64_t heads, int64_t heads_kv, int64_t D, 
         p.ws_ml = slots * rows_wg * W * 4;
         p.ws_prefix = p.ws_ml + slots * rows_wg * 8;
     }
-    p.bytes = p.ws_prefix + 8 * (B + 1);
+    const bool joined = p.tile ? p.splits > 1 : !p.whole;
+    p.bytes = joined ? p.ws_prefix + 8 * (B + 1) : 0;         // (nothing is parked without a join)
     *out = p;
     return FA_OK;
 }
@@ -308,14 +309,16 @@ int fa_cache_attn(const void* q, void* out, const void* k_cache, const void* v_c
         if (token_strides[i] % 8) return fail(FA_ERR_MISALIGNED, "rows of queries and output must be 16-byte aligned");
     }
     if (num_tokens == 0) return FA_OK;
-    if (!workspace || workspace_bytes < plan.bytes || !aligned(workspace, 16))
+    if (plan.bytes && (!workspace || workspace_bytes < plan.bytes || !aligned(workspace, 16)))
         return fail(FA_ERR_WORKSPACE, "fa_cache_attn: workspace must be 16-byte aligned and hold %lld bytes", (long long)plan.bytes);
     fa::CacheAttnParams p{};
     p.q = q; p.o = out; p.k = (const uint8_t*)k_cache; p.v = (const uint8_t*)v_cache; p.ks = k_scale; p.vs = v_scale;
     p.tables = block_tables; p.seq_lens = seq_lens; p.cu_q = cu_q;
-    p.ws_o = (float*)((char*)workspace + plan.ws_o);
-    p.ws_ml = (float*)((char*)workspace + plan.ws_ml);
-    p.ws_prefix = (long long*)((char*)workspace + plan.ws_prefix);
+    if (plan.bytes) {
+        p.ws_o = (float*)((char*)workspace + plan.ws_o);
+        p.ws_ml = (float*)((char*)workspace + plan.ws_ml);
+        p.ws_prefix = (long long*)((char*)workspace + plan.ws_prefix);
+    }
     p.q_st = token_strides[0]; p.q_sh = token_strides[1]; p.o_st = token_strides[2]; p.o_sh = token_strides[3];
     p.k_bs = block_strides[0]; p.v_bs = block_strides[1]; p.ks_bs = block_strides[2]; p.vs_bs = block_strides[3]; p.table_stride = table_stride;
     p.num_blocks = (int32_t)num_blocks; p.B = (int32_t)num_requests; p.T = (int32_t)num_tokens; p.Hq = (int32_t)heads; p.Hkv = (int32_t)heads_kv;

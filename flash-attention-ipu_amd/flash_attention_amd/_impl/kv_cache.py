@@ -235,7 +235,7 @@ def cache_append(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, k_cache:
 
 def _attn_call(q, k_cache, v_cache, k_scale, v_scale, block_tables, seq_lens, cu_q, softmax_scale, max_q_len, out):
     name = "flash_attention_cached"
-    key = (q.shape, q.stride(), q.dtype, out.shape, out.stride(), out.dtype, max_q_len, k_cache.shape, k_cache.stride(), v_cache.shape, v_cache.stride(), k_cache.dtype,
+    key = (q.shape, q.stride(), q.dtype, None if out is None else (out.shape, out.stride(), out.dtype), max_q_len, k_cache.shape, k_cache.stride(), v_cache.shape, v_cache.stride(), k_cache.dtype,
            v_cache.dtype, k_scale.shape, k_scale.stride(), v_scale.shape, v_scale.stride(), k_scale.dtype, v_scale.dtype, block_tables.shape, block_tables.stride(),
            block_tables.dtype, seq_lens.shape, seq_lens.stride(), seq_lens.dtype, cu_q.shape, cu_q.stride(), cu_q.dtype)
     lib = _native._LIB or _native.load_native_library()
@@ -245,7 +245,7 @@ def _attn_call(q, k_cache, v_cache, k_scale, v_scale, block_tables, seq_lens, cu
             raise TypeError(f"{name}: q must be float16 or bfloat16 (got {q.dtype})")
         if q.ndim != 3 or q.shape[1] < 1:
             raise ValueError(f"{name}: q must be [tokens, heads, head dim] (got {tuple(q.shape)})")
-        if out.shape != q.shape or out.dtype != q.dtype or out.stride(2) != 1 or out.stride(0) % 8 or out.stride(1) % 8:
+        if out is not None and (out.shape != q.shape or out.dtype != q.dtype or out.stride(2) != 1 or out.stride(0) % 8 or out.stride(1) % 8):
             raise ValueError(f"{name}: out must have q's shape and dtype and 16-byte rows")
         T, H, D = q.shape
         heads_kv = k_cache.shape[1] if k_cache.ndim == 4 else 0
@@ -265,30 +265,33 @@ def _attn_call(q, k_cache, v_cache, k_scale, v_scale, block_tables, seq_lens, cu
             _native._raise(int(nbytes))
         rows = q.stride(2) == 1 and q.stride(0) % 8 == 0 and q.stride(1) % 8 == 0
         known = _remember(key, ((B, T, H, heads_kv, D, W, N, P, width, table_stride, max_q_len), nbytes, rows,
-                                _i64x4((q.stride(0), q.stride(1), out.stride(0), out.stride(1))), _i64x4(strides), _native.FA_DTYPE[q.dtype]))
+                                _i64x4((q.stride(0), q.stride(1)) + (out.stride()[:2] if out is not None else (H * D, D))), _i64x4(strides), _native.FA_DTYPE[q.dtype]))
     sizes, nbytes, rows, tokens, strides, dtype = known
     dev = q.device
+    if out is None:
+        out = torch.empty(q.shape, dtype=q.dtype, device=dev)
     if not (q.is_cuda and dev == out.device == k_cache.device == v_cache.device == k_scale.device == v_scale.device == block_tables.device == seq_lens.device
             == cu_q.device):
         raise ValueError(f"{name}: all tensors must be on one GPU")
     if out.data_ptr() % 16:
         raise ValueError(f"{name}: out must be 16-byte aligned")
     if sizes[1] == 0:
-        return
+        return out
     if not rows or q.data_ptr() % 16:
         q = q.clone(memory_format=torch.contiguous_format)
         tokens = _i64x4((q.stride(0), q.stride(1), out.stride(0), out.stride(1)))
     # (a workspace of its own for every call: the allocator orders its reuse on the stream, and a captured graph keeps the one it was captured with)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
     stream, prev = _native.stream_of(dev)
     try:
         rc = lib.fa_cache_attn(q.data_ptr(), out.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), block_tables.data_ptr(),
-                               seq_lens.data_ptr(), cu_q.data_ptr(), ws.data_ptr(), nbytes, *sizes, tokens, strides, dtype, softmax_scale, stream)
+                               seq_lens.data_ptr(), cu_q.data_ptr(), None if ws is None else ws.data_ptr(), nbytes, *sizes, tokens, strides, dtype, softmax_scale, stream)
     finally:
         if prev >= 0:
             torch.cuda.set_device(prev)
     if rc != 0:
         _native._raise(rc)
+    return out
 
 
 @custom_op("flash_attention_amd::cached", mutates_args=("out",))
@@ -325,11 +328,12 @@ def flash_attention_cached(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torc
         raise ValueError(f"flash_attention_cached: softmax_scale must be finite and > 0 (got {softmax_scale})")
     if max_q_len is None:
         max_q_len = max(1, q.shape[0] - seq_lens.shape[0] + 1) if seq_lens.ndim == 1 else 1
-    if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    call = _attn_op if torch.compiler.is_compiling() else _attn_call
-    call(q, k_cache, v_cache, k_scale, v_scale, block_tables, seq_lens, cu_q, softmax_scale, max_q_len, out)
-    return out
+    if torch.compiler.is_compiling():
+        if out is None:
+            out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        _attn_op(q, k_cache, v_cache, k_scale, v_scale, block_tables, seq_lens, cu_q, softmax_scale, max_q_len, out)
+        return out
+    return _attn_call(q, k_cache, v_cache, k_scale, v_scale, block_tables, seq_lens, cu_q, softmax_scale, max_q_len, out)
 
 
 class KVCache:

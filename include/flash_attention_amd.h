@@ -345,7 +345,7 @@ int fa_cache_append(const void* k, const void* v, const int32_t* slots, void* k_
  * h / (heads / heads_kv).  Rows of out behind cu_q[num_requests] are not written.  Lengths and tables are read on the device only, and held inside the
  * tensors: no value in them leads to an access outside.  max_q_len: the longest run, as far as the caller knows: it chooses the kernel, and results are
  * right whatever it is.  The scales have to be >= 0.
- * workspace: fa_cache_attn_workspace() bytes (negative: an error code), 16-byte aligned, for this call alone while it runs.
+ * workspace: fa_cache_attn_workspace() bytes (negative: an error code; 0: none, it may be NULL), 16-byte aligned, for this call alone while it runs.
  * Partial sums are joined in a fixed order: results are bit-reproducible from call to call.
  */
 int64_t fa_cache_attn_workspace(int64_t num_requests, int64_t num_tokens, int64_t heads, int64_t heads_kv, int64_t D, int64_t block_size, int64_t max_blocks,

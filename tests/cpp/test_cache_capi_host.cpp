@@ -113,7 +113,7 @@ int main() {
         return fa_cache_attn(buf, buf, buf, buf, (float*)buf, (float*)buf, ip, ip, ip, buf, ws - short_by, B, T, H, Hk, D, W, N, P, width, width, most, t4, b4, dtype, scale, nullptr);
     };
     CHECK(attn(2, 2, 8, 2, 128, 10, 64, 5, 1, 0.1f, 0, 1) == FA_OK);
-    CHECK(attn(2, 2, 8, 2, 128, 10, 64, 5, 1, 0.1f, 1, 1) == FA_ERR_WORKSPACE);
+    CHECK(attn(2, 2, 8, 2, 128, 10, 64, 500, 1, 0.1f, 1, 1) == FA_ERR_WORKSPACE && attn(2, 2, 8, 2, 128, 10, 64, 500, 1, 0.1f, 0, 1) == FA_OK);
     CHECK(attn(2, 2, 8, 2, 128, 10, 64, 5, 1, 0.1f, 0, 2) == FA_ERR_BAD_DTYPE);
     CHECK(attn(2, 2, 8, 3, 128, 10, 64, 5, 1, 0.1f, 0, 1) == FA_ERR_BAD_SHAPE && attn(2, 2, 8, 2, 130, 10, 64, 5, 1, 0.1f, 0, 1) == FA_ERR_BAD_SHAPE);
     CHECK(attn(2, 2, 8, 2, 128, 10, 48, 5, 1, 0.1f, 0, 1) == FA_ERR_BAD_SHAPE && attn(0, 2, 8, 2, 128, 10, 64, 5, 1, 0.1f, 0, 1) == FA_ERR_BAD_SHAPE);
@@ -129,15 +129,16 @@ int main() {
             CHECK(attn(B, T, Hk * group, Hk, D, 10, 64, width, most, 0.1f, 0, 1) == FA_OK);
             const int64_t W = (D + 63) / 64 * 64;
             CHECK(g_plan.width == W && g_plan.grid >= 1 && g_attn.grid == g_plan.grid && (g_plan.ws_ml & 15) == 0 && (g_plan.ws_prefix & 7) == 0);
-            CHECK(g_plan.ws_prefix + 8 * (B + 1) <= g_plan.bytes);
+            const bool joined = g_plan.tile ? g_plan.splits > 1 : !g_plan.whole;
+            CHECK(joined ? g_plan.ws_prefix + 8 * (B + 1) <= g_plan.bytes : !g_attn.ws_o && !g_attn.ws_ml && !g_attn.ws_prefix);
             int64_t slots, rows;
             if (g_plan.tile) {
                 rows = 64 * g_plan.nr;
-                slots = g_plan.splits > 1 ? Hk * g_plan.max_tiles * g_plan.splits : 0;
+                slots = joined ? Hk * g_plan.max_tiles * g_plan.splits : 0;
                 CHECK(g_plan.grid == Hk * g_plan.max_tiles * g_plan.splits && g_plan.max_tiles >= (T * group + rows - 1) / rows);
             } else {
                 rows = 16 * g_plan.nr;
-                slots = g_plan.whole ? 0 : 2ll * g_plan.grid;
+                slots = !joined ? 0 : 2ll * g_plan.grid;
                 CHECK(g_plan.nr == 1 || W <= 128);
             }
             CHECK(g_plan.ws_ml - g_plan.ws_o >= slots * rows * W * 4 && g_plan.ws_prefix - g_plan.ws_ml >= slots * rows * 8);

@@ -25,7 +25,7 @@ def test_c_entry_points_refuse_before_they_launch():
 
     lib = _native.load_native_library()
     assert lib.fa_cache_attn_workspace(1, 1, 8, 3, 128, 64, 4, 1) == -2 and b"multiple of heads_kv" in lib.fa_last_error()
-    assert lib.fa_cache_attn_workspace(1, 1, 8, 2, 128, 64, 4, 1) > 0
+    assert lib.fa_cache_attn_workspace(1, 1, 8, 2, 128, 64, 400, 1) > 0 and lib.fa_cache_attn_workspace(1, 1, 8, 2, 128, 64, 4, 1) == 0
     assert lib.fa_cache_append(None, None, None, None, None, None, None, 1, 1, 64, 64, 1, 16, None, None, 1, None) == -1
     assert lib.fa_error_string(-16) == b"workspace too small"
 
