@@ -97,13 +97,14 @@ struct CacheAttnParams {
     int32_t whole;          // row kernel: no row tile is cut, none is joined
     int32_t splits;         // tile kernel: parts of a tile's key range
     int32_t max_tiles;      // tile kernel: bound on the row tiles of one key/value head
+    int32_t join_rows, join_chunks;   // join kernel: rows of a workgroup (1 .. 16), workgroups that share the rows of a tile
     float scale_log2;
 };
 struct CacheAttnPlan {
     int32_t tile;           // 0 = row kernel (few query rows per key/value head), 1 = tile kernel
     int32_t nr;             // 16-row query tiles per wave
     int32_t width;          // W
-    int32_t grid, splits, max_tiles, min_units, whole;
+    int32_t grid, splits, max_tiles, min_units, whole, join_rows, join_chunks;
     int64_t ws_o, ws_ml, ws_prefix, bytes;   // workspace offsets in bytes and its size
 };
 hipError_t launch_cache_attn(const CacheAttnParams& p, const CacheAttnPlan& plan, int dtype, hipStream_t stream);

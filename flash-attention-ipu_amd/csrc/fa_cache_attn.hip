@@ -36,6 +36,7 @@ namespace fa {
 namespace {
 
 typedef unsigned u32x2c __attribute__((ext_vector_type(2)));
+typedef float f32x2c __attribute__((ext_vector_type(2)));
 
 template <typename T> struct Code;
 template <> struct Code<__bf16> {
@@ -837,10 +838,12 @@ __global__ __launch_bounds__(256, W > 128 ? 1 : 2) void cache_tile_kernel(CacheA
     else st.park(p, ((long long)h * p.max_tiles + tile) * p.splits + part, ROWS, 16 * NR * wave, lane, sum, top);
 }
 
-// ---- join kernel: partial sums of one (request, key/value head, row tile), 64 columns per workgroup -------------------------------------------
-// slots in order, so that results are the same from call to call
+// ---- join kernel: partial sums of join_rows rows of one (request, key/value head, row tile), 64 columns per workgroup --------------------------
+// Bound: latency, of which the loads of a strand of slots are most; so few rows are spread over more workgroups of more strands, and a strand has
+// four slots' loads in flight.  The order of the sums is fixed by the layout: results are the same from call to call.
 template <typename T, bool TILE>
 __global__ __launch_bounds__(256) void cache_join_kernel(CacheAttnParams p, int W, int rows16) {
+    constexpr int DEEP = 4;
     __shared__ f32x4 part_o[256];
     __shared__ float part_m[256], part_l[256];
     int b, h, tile;
@@ -862,11 +865,12 @@ __global__ __launch_bounds__(256) void cache_join_kernel(CacheAttnParams p, int 
     } else {
         b = (int)blockIdx.x / p.Hkv;
         h = (int)blockIdx.x - b * p.Hkv;
-        tile = (int)blockIdx.y;
+        tile = (int)blockIdx.y / p.join_chunks;
     }
+    const int chunk = (int)blockIdx.y % p.join_chunks, tiles_y = (int)gridDim.y / p.join_chunks;
     const Request rq = request_of(p, b);
     const int rows = rq.n * p.group, tiles = (rows + rows16 - 1) / rows16, tid = (int)threadIdx.x;
-    for (; tile < tiles; tile += TILE ? tiles : (int)gridDim.y) {      // (more row tiles than the grid was told: every one is still reached)
+    for (; tile < tiles; tile += TILE ? tiles : tiles_y) {      // (more rows than the grid was told: every one is still reached)
         if constexpr (!TILE) {
             range = range_of(p, p.ws_prefix[p.B]);
             item0 = p.ws_prefix[b] + ((long long)h * tiles + tile) * rq.units;
@@ -875,24 +879,35 @@ __global__ __launch_bounds__(256) void cache_join_kernel(CacheAttnParams p, int 
             if (w0 == w1) continue;                                    // (finished by one workgroup)
         }
         // threads: strands of slots x rows x 16 groups of four columns
-        for (int base = 0; base < min(rows16, rows - tile * rows16); base += 16) {
-            const int live = min(16, rows - tile * rows16 - base);
+        const int there = min(rows16, rows - tile * rows16);
+        for (int base = chunk * p.join_rows; base < there; base += p.join_chunks * p.join_rows) {
+            const int live = min(p.join_rows, there - base);
             const int lanes = live > 8 ? 256 : live > 4 ? 128 : live > 2 ? 64 : live > 1 ? 32 : 16;
             const int strands = 256 / lanes, strand = tid / lanes, row = (tid % lanes) >> 4, c = tid & 15;
             const int col = 64 * (int)blockIdx.z + 4 * c;
             float top = -INFINITY, sum = 0.f;
             f32x4 o = {0.f, 0.f, 0.f, 0.f};
             if (row < live) {
-                for (long long w = w0 + strand; w <= w1; w += strands) {
-                    const long long slot = TILE ? slot0 + w : 2 * w + (w * range >= item0 ? 0 : 1);
-                    const long long at = slot * rows16 + base + row;
-                    const float m = p.ws_ml[2 * at], l = p.ws_ml[2 * at + 1];
-                    const f32x4 v = *(const f32x4*)(p.ws_o + at * W + col);
-                    const float now = __builtin_fmaxf(top, m), b0 = now == -INFINITY ? 0.f : now;
-                    const float f0 = fast_exp2(top - b0), f1 = fast_exp2(m - b0);
-                    o = o * f0 + v * f1;
-                    sum = sum * f0 + l * f1;
-                    top = now;
+                for (long long w = w0 + strand; w <= w1; w += DEEP * strands) {
+                    f32x2c ml[DEEP];
+                    f32x4 v[DEEP];
+#pragma unroll
+                    for (int j = 0; j < DEEP; ++j) {
+                        const long long wj = w + j * strands <= w1 ? w + j * strands : w;
+                        const long long slot = TILE ? slot0 + wj : 2 * wj + (wj * range >= item0 ? 0 : 1);
+                        const long long at = slot * rows16 + base + row;
+                        ml[j] = *(const f32x2c*)(p.ws_ml + 2 * at);
+                        v[j] = *(const f32x4*)(p.ws_o + at * W + col);
+                    }
+#pragma unroll
+                    for (int j = 0; j < DEEP; ++j) {
+                        if (w + j * strands > w1) continue;
+                        const float m = ml[j][0], now = __builtin_fmaxf(top, m), b0 = now == -INFINITY ? 0.f : now;
+                        const float f0 = fast_exp2(top - b0), f1 = fast_exp2(m - b0);
+                        o = o * f0 + v[j] * f1;
+                        sum = sum * f0 + ml[j][1] * f1;
+                        top = now;
+                    }
                 }
             }
             part_o[tid] = o;
@@ -942,7 +957,7 @@ hipError_t launch_typed(const CacheAttnParams& p, const CacheAttnPlan& plan, hip
     CacheAttnParams arg = p;
     int W = plan.width, rows = rows16;
     void* args[] = {&arg, &W, &rows};
-    const dim3 grid((unsigned)(p.Hkv * (plan.tile ? plan.max_tiles : p.B)), plan.tile ? 1u : (unsigned)plan.max_tiles, (unsigned)(plan.width / 64));
+    const dim3 grid((unsigned)(p.Hkv * (plan.tile ? plan.max_tiles : p.B)), (unsigned)(p.join_chunks * (plan.tile ? 1 : plan.max_tiles)), (unsigned)(plan.width / 64));
     return hipLaunchKernel(plan.tile ? (const void*)cache_join_kernel<T, true> : (const void*)cache_join_kernel<T, false>, grid, dim3(256), args, 0, stream);
 }
 

@@ -22,17 +22,18 @@ int fail(int code, const char* fmt, ...) {
 int launched(hipError_t e) { return e == hipSuccess ? FA_OK : fail(FA_ERR_LAUNCH, "kernel launch failed: %s", hipGetErrorString(e)); }
 
 constexpr int64_t kMaxCount = 1ll << 30;      // rows, items, tokens: 32-bit indexes with room for a grid's stride
+constexpr int64_t kMaxGrid = 1ll << 23;       // workgroups along x: times 256 threads stays below 2^32
 constexpr int64_t kMaxStride = 1ll << 40;     // elements: products with 32-bit indexes stay inside 64 bits
-constexpr int kWholeUnits = 16;               // 64-token units of a request up to which the row kernel cuts none
 constexpr int kCus = 256;                     // compute units of an MI355X: sizes grids, never correctness
 
 int64_t up(int64_t a, int64_t b) { return (a + b - 1) / b; }
 bool aligned(const void* p, uintptr_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0; }
 
 // ---- norm and rotation ------------------------------------------------------------------------------------------------------------------
-constexpr int kRopeMaxBlocks = 768;           // backward: workgroups per side = rows of partial weight gradients
-
-constexpr int kRopeFwdBlocks = 2048;          // forward: workgroups per side
+// Workgroups per side.  Backward: also the rows of partial weight gradients.  16384 tokens of 32 + 8 heads of 128 in bf16: 138 us with 256, 100 with 512, 101 with
+// 768, 105 with 1024; 2048 tokens 22.5, 20.7, 22.3, 24.9.  Forward: flat between 1024 and 4096 (59 .. 61 us; 512: 66).
+constexpr int kRopeMaxBlocks = 768;
+constexpr int kRopeFwdBlocks = 2048;
 
 struct RopeCall {
     fa::RopeParams p;
@@ -75,16 +76,16 @@ int rope_common(RopeCall* c, const void* q_weight, const void* k_weight, int32_t
     return FA_OK;
 }
 
-// Heads per lane group, items and workgroups of both sides.  Two heads per lane group fetch cosines, sines and position once and keep more loads in
-// flight ([4, 4096, 32 + 8, 128] bf16: 60.9 us, four heads 62.7), but a launch of few rows needs its lanes ([64, 32 + 8, 128]: 4.1 us with one).  What moves more
-// than the 256 MB of the last cache is read and written past it: forward 62.7 -> 60.9, backward 98.6 -> 91.8 us there; 50 MB that the next kernel
-// finds in the cache lose by it (forward 11.9 -> 13.7 us).
+// Heads per lane group, items and workgroups of both sides.  What moves more than the 256 MB of the last cache is read and written past it (16384 tokens of
+// 32 + 8 heads of 128 in bf16: forward 65.2 -> 60.4 us, backward 105 -> 100; 8192 tokens, 168 and 252 MB, lose by it: 30.3 -> 32.7 and 51.3 -> 55.4).  Two heads
+// per lane group fetch cosines, sines and position once and keep more loads in flight: 68.8 -> 60.3 us there, 62.3 -> 57.4 for 8192 tokens of 32-bit rows and
+// 10.5 -> 9.5 for 1024; 16-bit rows inside the cache want the lanes instead (4096 tokens: 17.8 us with one, 19.5 with two).  Four heads: 62.7.
 void rope_shape(RopeCall* c, int64_t B, bool backward) {
     fa::RopeParams& p = c->p;
     const int lpr = c->vec ? p.D * c->es / 32 : 64;
     const int64_t tokens = B * p.L, rows = tokens * (p.side[0].heads + p.side[1].heads);
-    c->hc = c->vec && rows * lpr / 64 >= 8192 ? 2 : 1;
     c->stream_past = rows * p.D * c->es * (backward ? 3 : 2) > (256ll << 20);
+    c->hc = c->vec && (c->es == 4 || c->stream_past) ? 2 : 1;
     for (fa::RopeSide& s : p.side) {
         s.chunks = (int32_t)up(s.heads, c->hc);
         s.items = (int32_t)(tokens * s.chunks);
@@ -128,14 +129,21 @@ int attn_plan(int64_t B, int64_t T, int64_t heads, int64_t heads_kv, int64_t D, 
     if (max_q_len > T) max_q_len = T > 0 ? T : 1;
     const int64_t rows = max_q_len * group, max_units = up(max_blocks * block_size, 64);
     p.width = (int32_t)W;
-    p.tile = rows > 32;
+    // The row kernel reads the cache once per row tile: 32 rows, 16 above width 128.  64 requests of 2048 tokens, 8 heads, row kernel against tile kernel: width 64:
+    // 64 rows 53 to 65 us, 128 rows 101 to 67; width 128: 32 rows 58 to 86, 48 rows 110 to 87; width 256: 16 rows 108 to 171, 24 rows 200 to 172.
+    // (One request of 16384: 17.5 to 22.6 and 20.4 to 23.9; 24 to 31 and 26 to 31; 29 to 35 and 35 to 34.)
+    p.tile = rows > (W == 64 ? 64 : W == 128 ? 32 : 16);
     p.min_units = 4;
     if (!p.tile) {
-        p.nr = rows > 16 && W <= 128 ? 2 : 1;
+        // 32 rows in one pass or 16 in each of two (64 requests of 2048: 20 rows of width 128 57 to 88 us); for up to 16 rows the smaller tile (49 to 55)
+        p.nr = rows > 16 ? 2 : 1;
         p.max_tiles = (int32_t)up(rows, 16 * p.nr);
-        int64_t grid = W > 64 || p.nr > 1 ? 2 * kCus : 3 * kCus;
-        // short caches: four waves are through a row's units in a few rounds, which is less than a second launch takes
-        p.whole = max_units <= kWholeUnits;
+        // two resident workgroups per compute unit (64 requests of 4096, width 128: 86.4 us; one 89, three 104, four 97; width 64: 45.6, 49.1, 52.3, 49.3);
+        // at least four units for each, a round of its waves (one request of 8192: 13.9 us; one unit 14.5, eight 15.3)
+        int64_t grid = 2 * kCus;
+        // short caches: four waves are through a row's units in a few rounds, which is less than a second launch takes (one request of 1024 tokens, whole against
+        // cut: width 64 8.5 to 10.6 us, 128 11.5 to 12.1, 256 21 to 16.9; of 512: 16.3 to 17.5 there; of 2048: 12.1 to 10.6, 17 to 12.6)
+        p.whole = max_units <= (W <= 128 ? 16 : 8);
         if (p.whole) p.min_units = 1;
         const int64_t most = p.whole ? B * heads_kv * p.max_tiles : up(B * heads_kv * p.max_tiles * max_units, p.min_units);
         if (grid > most) grid = most;
@@ -147,14 +155,18 @@ int attn_plan(int64_t B, int64_t T, int64_t heads, int64_t heads_kv, int64_t D, 
         p.ws_prefix = p.ws_ml + slots * 16 * p.nr * 8;
     } else {
         p.nr = W <= 128 ? 2 : 1;
-        const int64_t rows_wg = 64 * p.nr, tiles = up(T * group, rows_wg), bound = T * group / rows_wg + B;
-        int64_t splits = 1;
-        if (tiles * heads_kv < kCus) {
-            splits = 2 * kCus / (tiles * heads_kv);
-            if (splits > 16) splits = 16;
-            if (splits > up(max_units, 4)) splits = up(max_units, 4);
-        }
-        if (bound * heads_kv * splits > (1ll << 30)) return fail(FA_ERR_TOO_LARGE, "more than 2^30 row tiles");
+        const int64_t rows_wg = 64 * p.nr, bound = T * group / rows_wg + B;
+        int64_t tiles = up(T * group, rows_wg);
+        if (tiles < B) tiles = B;                 // (a request with tokens has a tile of its own)
+        // Too few workgroups for the chip: the key range is cut until each compute unit has as many as it holds (two, one above width 128), down to parts of two
+        // units, or of sixteen where every compute unit has a workgroup already.  Width 128, 1 / 2 / 4 / 8 / 16 / 32 parts: 64 tokens of group 4 over 16384: 428 225
+        // 120 69 47 44 us; 512 over 8192: 215 125 94 105 129 182; twice 512 over 8192: 222 166 171; 8 times 128 over 1024: 37 44 55; 256 over 512: 22 21 20 24.
+        const int64_t wgs = tiles * heads_kv, parts = up(max_units, wgs < kCus ? 2 : 16);
+        int64_t splits = (W <= 128 ? 2 : 1) * kCus / wgs;
+        if (splits > 32) splits = 32;
+        if (splits > parts) splits = parts;
+        if (splits < 1) splits = 1;
+        if (bound * heads_kv * splits > kMaxGrid) return fail(FA_ERR_TOO_LARGE, "more than 2^23 row tiles");
         p.max_tiles = (int32_t)bound;
         p.splits = (int32_t)splits;
         p.grid = (int32_t)(bound * heads_kv * splits);
@@ -163,6 +175,12 @@ int attn_plan(int64_t B, int64_t T, int64_t heads, int64_t heads_kv, int64_t D, 
         p.ws_prefix = p.ws_ml + slots * rows_wg * 8;
     }
     const bool joined = p.tile ? p.splits > 1 : !p.whole;
+    if (!p.tile && joined && B * heads_kv > kMaxGrid) return fail(FA_ERR_TOO_LARGE, "more than 2^23 requests times key/value heads");
+    // (the join wants a workgroup per compute unit: eight tokens over 16384, width 128: 28.8 us with a quarter of that, 23.6; eight times as many 24.3)
+    const int64_t tile_rows = (p.tile ? 64 : 16) * p.nr, most_rows = rows < tile_rows ? rows : tile_rows, items = heads_kv * (p.tile ? p.max_tiles : B * p.max_tiles) * (W / 64);
+    p.join_rows = 16;
+    while (p.join_rows > 1 && items * up(most_rows, p.join_rows) < kCus) p.join_rows /= 2;
+    p.join_chunks = (int32_t)up(most_rows, p.join_rows);
     p.bytes = joined ? p.ws_prefix + 8 * (B + 1) : 0;         // (nothing is parked without a join)
     *out = p;
     return FA_OK;
@@ -248,7 +266,8 @@ int fa_cache_tables(const int32_t* seq_lens, const int32_t* new_lens, int32_t* b
     p.seq_in = seq_lens; p.new_lens = new_lens; p.tables = block_tables; p.pool = free_blocks; p.free_in = free_count; p.free_out = free_count_out;
     p.seq_out = seq_lens_out; p.cu_new = cu_new; p.granted = granted; p.positions = positions; p.slots = slots; p.table_stride = table_stride;
     p.B = (int32_t)num_requests; p.width = (int32_t)max_blocks; p.T = (int32_t)num_tokens; p.shift = shift; p.pool_size = (int32_t)pool_size;
-    // one launch while a workgroup places the tokens in a few rounds (a second launch costs more than four rounds of 1024 tokens)
+    // one launch while a workgroup places the tokens in a few rounds of 1024 (64 requests: 1024 tokens 6.9 us, with a second launch 9.2; 4096: 9.1 to 9.3; 8192: 11.9 to
+    // 9.5; one request: 4.4 to 6.2, 5.2 to 6.3, 6.4 to 6.5)
     p.fused = num_tokens <= 4096;
     return launched(fa::launch_cache_tables(p, (hipStream_t)stream));
 }
@@ -260,7 +279,7 @@ int fa_cache_append(const void* k, const void* v, const int32_t* slots, void* k_
     if (dtype != FA_DTYPE_F16 && dtype != FA_DTYPE_BF16) return fail(FA_ERR_BAD_DTYPE, "keys and values must be FA_DTYPE_F16 or FA_DTYPE_BF16 (got %d)", dtype);
     if (int rc = cache_geometry(num_blocks, heads_kv, block_size, D, W, block_strides, k_cache, v_cache)) return rc;
     if (num_tokens < 0) return fail(FA_ERR_BAD_SHAPE, "num_tokens must be >= 0");
-    if (num_tokens > kMaxCount) return fail(FA_ERR_TOO_LARGE, "more than 2^30 tokens");
+    if (num_tokens > 64 * kMaxGrid) return fail(FA_ERR_TOO_LARGE, "more than 2^29 tokens");
     if (!aligned(k, 16) || !aligned(v, 16)) return fail(FA_ERR_MISALIGNED, "keys and values must be 16-byte aligned");
     for (int i = 0; i < 4; ++i) {
         if (token_strides[i] < 0 || token_strides[i] >= kMaxStride) return fail(FA_ERR_BAD_STRIDE, "stride %lld is negative or too large", (long long)token_strides[i]);
@@ -275,12 +294,12 @@ int fa_cache_append(const void* k, const void* v, const int32_t* slots, void* k_
     }
     p.T = (int32_t)num_tokens; p.H = (int32_t)heads_kv; p.D = (int32_t)D; p.W = (int32_t)W; p.shift = block_shift(block_size);
     p.limit = num_blocks * block_size;
-    // tokens per workgroup: about 2048 workgroups in all, so that steps of single tokens spread over the chip (a wave per run) and prompts do
-    // not pay for workgroups in which no run begins
+    // tokens per workgroup: about 1024 workgroups in all, which the chip holds at once.  Steps of single tokens spread over the chip (64 tokens of 8 heads of 128: 5.5 us
+    // with 4, 15 with 16, 50 with 64), prompts do not pay for workgroups in which no run begins (16384 tokens: 204 us with 4, 59 with 16, 27 with 64;
+    // 2048: 30, 11.8 and 8.5).
     int window = 4;
-    while (window < 64 && up(num_tokens, window) * 2 * heads_kv > 2048) window *= 2;
+    while (window < 64 && up(num_tokens, window) * 2 * heads_kv > 1024) window *= 2;
     p.window = window;
-    if (up(num_tokens, window) > 0x7fffffffll) return fail(FA_ERR_TOO_LARGE, "too many tokens");
     return launched(fa::launch_cache_append(p, dtype, (hipStream_t)stream));
 }
 
@@ -323,7 +342,7 @@ int fa_cache_attn(const void* q, void* out, const void* k_cache, const void* v_c
     p.k_bs = block_strides[0]; p.v_bs = block_strides[1]; p.ks_bs = block_strides[2]; p.vs_bs = block_strides[3]; p.table_stride = table_stride;
     p.num_blocks = (int32_t)num_blocks; p.B = (int32_t)num_requests; p.T = (int32_t)num_tokens; p.Hq = (int32_t)heads; p.Hkv = (int32_t)heads_kv;
     p.group = (int32_t)(heads / heads_kv); p.D = (int32_t)D; p.width = (int32_t)max_blocks; p.shift = block_shift(block_size);
-    p.grid = plan.grid; p.min_units = plan.min_units; p.whole = plan.whole; p.splits = plan.splits; p.max_tiles = plan.max_tiles;
+    p.grid = plan.grid; p.min_units = plan.min_units; p.whole = plan.whole; p.splits = plan.splits; p.max_tiles = plan.max_tiles; p.join_rows = plan.join_rows; p.join_chunks = plan.join_chunks;
     p.scale_log2 = softmax_scale * 1.44269504088896340736f;
     return launched(fa::launch_cache_attn(p, plan, dtype, (hipStream_t)stream));
 }

@@ -216,8 +216,8 @@ __global__ __launch_bounds__(kSlotThreads) void cache_slots_kernel(TablesParams 
 // Scales are powers of two because codes carry their own exponent: x / scale is exact, growing a scale only moves the codes' exponents (exact
 // but for what falls under the smallest code), and nothing is gained by filling the last fraction of the top binade.
 // Bound: memory (2 bytes in, 1 byte out per value) for prompts, latency for a step.  A workgroup owns `window` tokens of one head and cache;
-// the runs that begin in them are its work - a run is never shared, so scales need no atomics.  Long runs are taken by the whole workgroup,
-// several short ones by a wave each.
+// the runs that begin in them are its work - a run is never shared, so scales need no atomics.  One or two long runs are taken by the whole workgroup,
+// others by a wave each.
 // A work item is eight columns of four consecutive tokens: 16-byte loads, the values stay in registers between the maximum and the codes, and
 // both layouts store whole words - eight bytes of a key row, or (columns down the lanes) four tokens of a value column.
 typedef float f32x2 __attribute__((ext_vector_type(2)));
@@ -442,12 +442,10 @@ __global__ __launch_bounds__(256) void cache_append_kernel(AppendParams p) {
     }
     unsigned long long begins = __ballot(place[0] && !on[0] && lane < p.window);
     const unsigned long long on0 = __ballot(on[0]), on1 = __ballot(on[1]), on2 = __ballot(on[2]);
-    // one or two runs in a window of 16 tokens and more are long: the whole workgroup takes them; else a wave per run
-    const bool together = p.window >= 16 && __popcll(begins) <= 2;
+    const bool few = __popcll(begins) <= 2;
     for (int r = 0; begins; ++r) {
         const int i = __builtin_ctzll(begins);
         begins &= begins - 1;
-        if (!together && (r & 3) != wave) continue;
         const auto ones = [](unsigned long long m) { return ~m ? (int)__builtin_ctzll(~m) : 64; };
         int n = 1 + (i < 63 ? min(ones(on0 >> (i + 1)), 63 - i) : 0);
         if (n == 64 - i) {
@@ -455,6 +453,8 @@ __global__ __launch_bounds__(256) void cache_append_kernel(AppendParams p) {
             n += more;
             if (more == 64) n += ones(on2);
         }
+        const bool together = few && n >= 16;     // (of several runs, or for a short one, a wave each: 512 tokens of one request 6.7 us, 10.5 without)
+        if (!together && (r & 3) != wave) continue;
         const int t0 = t_first + i, slot = __builtin_amdgcn_readfirstlane(p.slots[t0]);
         const int64_t block = slot >> p.shift;
         const int off = slot & (P - 1);
