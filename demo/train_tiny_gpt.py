@@ -5,7 +5,10 @@ repository does not rebuild; only "does a model train through the HIP forward + 
 The task is learnable only through attention: token t+1 = (token t + token at the start of its 16-token
 segment) mod V, so the loss falls well below log(V) only if gradients flow through the causal attention.
 
-    python demo/train_tiny_gpt.py [--steps 60] [--block 256] [--no-override]
+    python demo/train_tiny_gpt.py [--steps 60] [--block 256] [--no-override] [--rotary]
+
+--rotary: normed and rotated heads, two key/value heads for four query heads, and at the end a continuation of held-out
+prompts over the 8-bit block cache.
 """
 import argparse
 import pathlib
@@ -32,12 +35,12 @@ def make_batch(batch, block, vocab, gen):
     return x[:, :-1].contiguous(), x[:, 1:].contiguous()
 
 
-def train(steps=60, block=256, batch=16, vocab=64, override=True, seed=0, log=None):
+def train(steps=60, block=256, batch=16, vocab=64, override=True, seed=0, log=None, rotary=False, keep=None):
     if override:
         import flash_attention_amd.auto  # noqa: F401
     torch.manual_seed(seed)
     gen = torch.Generator().manual_seed(seed)
-    model = TinyGPT(vocab=vocab, block=block, n_layer=2, n_head=4, n_embd=256).cuda()
+    model = TinyGPT(vocab=vocab, block=block, n_layer=2, n_head=4, n_embd=256, **(dict(rotary=True, n_kv_head=2) if rotary else {})).cuda()
     opt = torch.optim.AdamW(model.parameters(), lr=3e-3, weight_decay=0.0)
     losses = []
     for step in range(steps):
@@ -52,6 +55,8 @@ def train(steps=60, block=256, batch=16, vocab=64, override=True, seed=0, log=No
         losses.append(loss.item())
         if log and (step % 10 == 0 or step == steps - 1):
             log(f"step {step:3d}  loss {loss.item():.4f}")
+    if keep is not None:
+        keep.append(model)
     return losses
 
 
@@ -60,9 +65,18 @@ def main():
     ap.add_argument("--steps", type=int, default=60)
     ap.add_argument("--block", type=int, default=256)
     ap.add_argument("--no-override", action="store_true")
+    ap.add_argument("--rotary", action="store_true")
     a = ap.parse_args()
-    losses = train(a.steps, a.block, override=not a.no_override, log=print)
+    keep = []
+    losses = train(a.steps, a.block, override=not a.no_override, log=print, rotary=a.rotary, keep=keep)
     print(f"first {losses[0]:.3f} -> last {losses[-1]:.3f}  (log V = {torch.log(torch.tensor(64.0)).item():.3f})")
+    if a.rotary:
+        x, _ = make_batch(4, a.block, 64, torch.Generator().manual_seed(1))
+        lens = [a.block // 2 + 4 * i + 1 for i in range(4)]          # (their next tokens are inside a segment: the task defines them)
+        with torch.autocast("cuda", dtype=torch.bfloat16):
+            got = keep[0].eval().generate([r[:n].cuda() for r, n in zip(x, lens)], 3).cpu()
+        want = torch.stack([r[n:n + 3] for r, n in zip(x, lens)])
+        print(f"continuations: {int((got == want).sum())} of {want.numel()} tokens are the task's")
 
 
 if __name__ == "__main__":
