@@ -279,7 +279,7 @@ int fa_cache_append(const void* k, const void* v, const int32_t* slots, void* k_
     if (dtype != FA_DTYPE_F16 && dtype != FA_DTYPE_BF16) return fail(FA_ERR_BAD_DTYPE, "keys and values must be FA_DTYPE_F16 or FA_DTYPE_BF16 (got %d)", dtype);
     if (int rc = cache_geometry(num_blocks, heads_kv, block_size, D, W, block_strides, k_cache, v_cache)) return rc;
     if (num_tokens < 0) return fail(FA_ERR_BAD_SHAPE, "num_tokens must be >= 0");
-    if (num_tokens > 64 * kMaxGrid) return fail(FA_ERR_TOO_LARGE, "more than 2^29 tokens");
+    if (num_tokens > kMaxCount || num_tokens * heads_kv > 32 * kMaxGrid) return fail(FA_ERR_TOO_LARGE, "more than 2^28 rows of keys");
     if (!aligned(k, 16) || !aligned(v, 16)) return fail(FA_ERR_MISALIGNED, "keys and values must be 16-byte aligned");
     for (int i = 0; i < 4; ++i) {
         if (token_strides[i] < 0 || token_strides[i] >= kMaxStride) return fail(FA_ERR_BAD_STRIDE, "stride %lld is negative or too large", (long long)token_strides[i]);

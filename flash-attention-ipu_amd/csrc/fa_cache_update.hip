@@ -286,8 +286,10 @@ __device__ __forceinline__ void transpose4(unsigned (&r)[4]) {
     r[3] = __builtin_amdgcn_perm(d, b, 0x07060302u);
 }
 
-// one run: tokens t0 .. t0 + n - 1 into positions off .. off + n - 1 of a block.  NT = 64 (a wave) or 256 (the workgroup)
-template <typename T, int W, bool KEYS, int NT>
+// One run: tokens t0 .. t0 + n - 1 into positions off .. off + n - 1 of a block.  NT = 64 (a wave) or 256 (the workgroup).
+// HOLD: items per thread that stay in registers between the maximum and the codes: one where a whole block is one item per thread of a workgroup
+// (16384 tokens in blocks of 64, 8 heads of 128: 30.4 us, with two 32.0; of 64: 17.0 and 18.8), else two (blocks of 128: 26.3 us, with one 28.9).
+template <typename T, int W, int HOLD, bool KEYS, int NT>
 __device__ __forceinline__ void append_run(const AppendParams& p, int t0, int n, int64_t block, int off, int head, unsigned* shared_max) {
     constexpr int S = KEYS ? 0 : 1, WC = W / 8;                           // column chunks of a row
     const int tid = (int)threadIdx.x & (NT - 1);
@@ -300,7 +302,7 @@ __device__ __forceinline__ void append_run(const AppendParams& p, int t0, int n,
     const T* x = (const T*)p.x[S] + (int64_t)head * p.x_sh[S] + (int64_t)t0 * st;
     uint8_t* tile = (uint8_t*)p.cache[S] + block * p.block_stride[S] + (int64_t)head * P * W;
     float* scale = p.scale[S] + block * p.scale_stride[S] + head;
-    const float old = off ? *scale : 0.f;
+    float old = off ? *scale : 0.f;
 
     const auto place = [&](int i, int& g, int& c) {                       // item i: position group g, column chunk c
         if (KEYS) { g = g0 + i / WC; c = i % WC; }
@@ -334,7 +336,6 @@ __device__ __forceinline__ void append_run(const AppendParams& p, int t0, int n,
             }
         return m;
     };
-    constexpr int HOLD = 2;                    // items per thread that stay in registers between the two passes
     u32x4v held[HOLD][4];
     const auto over_all = [&](auto f) {
         u16x2 m = {0, 0};
@@ -358,6 +359,7 @@ __device__ __forceinline__ void append_run(const AppendParams& p, int t0, int n,
 #pragma unroll
     for (int h = 0; h < HOLD; ++h)
         if (tid + h * NT < items) load(tid + h * NT, held[h]);
+    asm volatile("" : "+v"(old));             // (here, before the maximum's barrier: the first thread stores the scale behind it)
     unsigned largest = over_all(look);
     const bool finite = largest < Bits<T>::top;
     if (!finite) largest = over_all(look_finite);
@@ -374,7 +376,7 @@ __device__ __forceinline__ void append_run(const AppendParams& p, int t0, int n,
         __threadfence();                       // these stores are done before the run's own bytes are written
         if constexpr (NT == 256) __syncthreads();
     }
-    if (tid == 0) *scale = now;                // (everyone has read the old one: it went into the maximum's round)
+    if (tid == 0) *scale = now;
     // a power of two that the conversion takes, and nothing but finite values
     const unsigned nb = __builtin_bit_cast(unsigned, now);
     const bool fast = finite && (nb & 0x807fffffu) == 0u && nb != 0u && nb != 0x7f800000u;
@@ -423,13 +425,15 @@ __device__ __forceinline__ void append_run(const AppendParams& p, int t0, int n,
     }
 }
 
-template <typename T, int W>
+template <typename T, int W, int HOLD>
 __global__ __launch_bounds__(256) void cache_append_kernel(AppendParams p) {
     __shared__ unsigned shared_max[4];
     const int lane = (int)threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-    const int head = (int)blockIdx.y >> 1;
-    const bool keys = ((int)blockIdx.y & 1) == 0;
-    const int P = 1 << p.shift, t_first = (int)blockIdx.x * p.window;
+    // all windows of the keys, then of the values; the heads of a window side by side, which read neighbouring pieces of its rows (41.0 -> 39.7 us)
+    const int half = (int)gridDim.x >> 1;
+    const bool keys = (int)blockIdx.x < half;
+    const int id = keys ? (int)blockIdx.x : (int)blockIdx.x - half, head = id % p.H;
+    const int P = 1 << p.shift, t_first = id / p.H * p.window;
     // Every wave finds the window's runs by itself, from loads that are in flight together: for the window's tokens and the 128 behind them, whether a
     // token goes on from its predecessor; a token with a place that does not begins a run, and the ones behind its bit are its length (P <= 128).
     bool place[3], on[3];
@@ -459,11 +463,11 @@ __global__ __launch_bounds__(256) void cache_append_kernel(AppendParams p) {
         const int64_t block = slot >> p.shift;
         const int off = slot & (P - 1);
         if (together) {
-            if (keys) append_run<T, W, true, 256>(p, t0, n, block, off, head, shared_max);
-            else append_run<T, W, false, 256>(p, t0, n, block, off, head, shared_max);
+            if (keys) append_run<T, W, HOLD, true, 256>(p, t0, n, block, off, head, shared_max);
+            else append_run<T, W, HOLD, false, 256>(p, t0, n, block, off, head, shared_max);
         } else {
-            if (keys) append_run<T, W, true, 64>(p, t0, n, block, off, head, shared_max);
-            else append_run<T, W, false, 64>(p, t0, n, block, off, head, shared_max);
+            if (keys) append_run<T, W, HOLD, true, 64>(p, t0, n, block, off, head, shared_max);
+            else append_run<T, W, HOLD, false, 64>(p, t0, n, block, off, head, shared_max);
         }
     }
 }
@@ -478,11 +482,14 @@ hipError_t launch_cache_tables(const TablesParams& p, hipStream_t stream) {
 }
 
 hipError_t launch_cache_append(const AppendParams& p, int dtype, hipStream_t stream) {
-    const dim3 grid((unsigned)((p.T + p.window - 1) / p.window), (unsigned)(2 * p.H));
+    const dim3 grid((unsigned)((p.T + p.window - 1) / p.window) * 2u * (unsigned)p.H);
     const auto kernel = [&](auto t) {
         using T = decltype(t);
-        return p.W == 64 ? (const void*)cache_append_kernel<T, 64> : p.W == 128 ? (const void*)cache_append_kernel<T, 128>
-             : p.W == 192 ? (const void*)cache_append_kernel<T, 192> : (const void*)cache_append_kernel<T, 256>;
+        const bool two = (p.W << p.shift) > 8192;
+        return p.W == 64 ? (const void*)cache_append_kernel<T, 64, 1>
+             : p.W == 128 ? (two ? (const void*)cache_append_kernel<T, 128, 2> : (const void*)cache_append_kernel<T, 128, 1>)
+             : p.W == 192 ? (two ? (const void*)cache_append_kernel<T, 192, 2> : (const void*)cache_append_kernel<T, 192, 1>)
+                          : (two ? (const void*)cache_append_kernel<T, 256, 2> : (const void*)cache_append_kernel<T, 256, 1>);
     };
     return launch1(dtype == 0 ? kernel(_Float16{}) : kernel(__bf16{}), grid, dim3(256), 0, stream, p);
 }
