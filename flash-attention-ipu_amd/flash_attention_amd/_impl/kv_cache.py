@@ -172,7 +172,7 @@ def _check_cache(name, k_cache, v_cache, k_scale, v_scale, heads_kv, D):
 
 def _append_call(k, v, slots, k_cache, v_cache, k_scale, v_scale):
     name = "cache_append"
-    key = (k.shape, k.stride(), v.shape, v.stride(), k.dtype, v.dtype, slots.shape, slots.dtype, k_cache.shape, k_cache.stride(), v_cache.shape, v_cache.stride(),
+    key = (k.shape, k.stride(), v.shape, v.stride(), k.dtype, v.dtype, slots.shape, slots.stride(), slots.dtype, k_cache.shape, k_cache.stride(), v_cache.shape, v_cache.stride(),
            k_cache.dtype, v_cache.dtype, k_scale.shape, k_scale.stride(), v_scale.shape, v_scale.stride(), k_scale.dtype, v_scale.dtype)
     known = _LAYOUTS.get(key)
     if known is None:
@@ -228,6 +228,8 @@ def cache_append(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, k_cache:
     largest value; later runs raise it where they need to, and the block's codes are brought along.  inf and NaN are stored as NaN.  One call may bring
     one run to a block: two runs in one block, or a slot twice, leave that block's contents unspecified.
     """
+    if torch.is_grad_enabled() and (k.requires_grad or v.requires_grad):
+        raise ValueError("cache_append has no gradient: call it under torch.no_grad()")
     if torch.compiler.is_compiling():
         return _append_op(k, v, slots, k_cache, v_cache, k_scale, v_scale)
     return _append_call(k, v, slots, k_cache, v_cache, k_scale, v_scale)

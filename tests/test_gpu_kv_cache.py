@@ -371,6 +371,44 @@ def test_large_scores_and_scales(kv, dtype):
     assert bool((out[1] == 0).all())
 
 
+@BOTH
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_more_rows_than_the_call_was_told_of(kv, dtype, D):
+    """parts of many row tiles that are joined although max_q_len said one row, and one tile although it said many"""
+    check_attention(kv, [3000, 10, 700], [40, 3, 1], 1, 4, D, 64, dtype, seed=21, max_q_len=1)
+    check_attention(kv, [9000], [12], 2, 2, D, 16, dtype, seed=22, max_q_len=1)
+    check_attention(kv, [5000, 0], [1, 2], 1, 2, D, 128, dtype, seed=23, max_q_len=500)
+
+
+@BOTH
+@pytest.mark.parametrize("D,group,new", [(64, 8, 8), (64, 16, 3), (128, 8, 4), (256, 4, 4)])
+def test_as_many_rows_as_the_row_kernel_takes(kv, dtype, D, group, new):
+    check_attention(kv, [6000, 5], [new, new], 1, group, D, 64, dtype, seed=24)
+    check_attention(kv, [6000, 5], [new + 1, new], 1, group, D, 64, dtype, seed=25)
+
+
+@BOTH
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("held,new", [([3000], [64]), ([2900, 0], [200, 30]), ([100], [300]), ([1500] * 3 + [0], [70, 1, 33, 129])])
+def test_prompts_in_parts(kv, dtype, D, held, new):
+    """few row tiles: their keys are cut into parts, more of them than a short request has units"""
+    check_attention(kv, held, new, 1, 2, D, 64, dtype, seed=26)
+
+
+def test_a_layout_is_looked_at_in_every_call(kv):
+    """the same shapes with other strides, after a call that passed"""
+    layer = kv.KVCache(1, 8, 2, 64, requests=2, max_tokens=64, block_size=16)._layer[0]
+    k = torch.zeros(4, 2, 64, dtype=torch.float16, device=DEV)
+    kv.cache_append(k, k, ints([0, 1, 2, 3]), *layer)
+    for slots in (ints([0, 9, 1, 9, 2, 9, 3, 9])[::2], ints([0]).expand(4)):
+        with pytest.raises(ValueError):
+            kv.cache_append(k, k, slots, *layer)
+    with pytest.raises(ValueError, match="no gradient"):
+        kv.cache_append(k.clone().requires_grad_(), k, ints([0, 1, 2, 3]), *layer)
+    with torch.no_grad():
+        kv.cache_append(k.clone().requires_grad_(), k, ints([0, 1, 2, 3]), *layer)
+
+
 def test_offsets_behind_32_bits(kv):
     """blocks that begin behind 4 GiB of codes"""
     N, H, P, D = 70000, 8, 64, 128
