@@ -22,7 +22,7 @@
 //                grid is fixed; the units of all (request, head, row tile) are one line that is cut into equal ranges on the device, from the
 //                lengths there: no length is known to the host, and one long request fills the chip.  A (request, head, row tile) inside one range
 //                is finished there; one that crosses ranges leaves unnormalised partial sums that the join kernel adds in order.
-//   tile kernel  128 rows per workgroup, 64 above head dim 128 (prompts): bound by the matrix pipe.  Four waves share a unit's operands,
+//   tile kernel  128 rows per workgroup, 64 where no request has more (prompts): bound by the matrix pipe.  Four waves share a unit's operands,
 //                converted once into LDS in the very order in which the lanes read them.  Grids too small for the chip cut every tile's
 //                key range into `splits` parts.
 // Stale codes behind a request's end are cleared before they meet a zero weight (0 * NaN), and a NaN code that only some rows of a unit may
@@ -688,13 +688,10 @@ __device__ __forceinline__ void mix() {
     }
 }
 
-// query tiles of 16 rows per wave: two where O (16 NR W / 64 registers) leaves room for two waves per SIMD
-constexpr int tile_nr(int W) { return W <= 128 ? 2 : 1; }
-
 // ---- tile kernel --------------------------------------------------------------------------------------------------------------------------
-template <typename T, int W, bool SMALL>
+template <typename T, int W, int NR, bool SMALL>
 __global__ __launch_bounds__(256, W > 128 ? 1 : 2) void cache_tile_kernel(CacheAttnParams p) {
-    constexpr int NR = tile_nr(W), ROWS = 64 * NR, NK = W / 64, ND = W / 16, NC = W / 32, KPW = NK, VPW = ND / 4;
+    constexpr int ROWS = 64 * NR, NK = W / 64, ND = W / 16, NC = W / 32, KPW = NK, VPW = ND / 4;
     using State = RowState<T, W, NR>;
     using vec8 = typename State::vec8;
     __shared__ u32x4 lds_k[2][4 * NC * 64], lds_v[2][2 * ND * 64];
@@ -944,7 +941,8 @@ template <typename T, int W>
 hipError_t launch_width(const CacheAttnParams& p, const CacheAttnPlan& plan, hipStream_t stream) {
     const bool small = p.shift < 6;
     const void* k;
-    if (plan.tile) k = small ? (const void*)cache_tile_kernel<T, W, true> : (const void*)cache_tile_kernel<T, W, false>;
+    if (plan.tile) k = plan.nr == 1 ? (small ? (const void*)cache_tile_kernel<T, W, 1, true> : (const void*)cache_tile_kernel<T, W, 1, false>)
+                                    : (small ? (const void*)cache_tile_kernel<T, W, 2, true> : (const void*)cache_tile_kernel<T, W, 2, false>);
     else k = plan.nr == 1 || W > 128 ? rows_kernel<T, W, 1>(p.shift) : rows_kernel<T, (W <= 128 ? W : 128), 2>(p.shift);
     return launch1(k, dim3((unsigned)plan.grid), dim3(256), 0, stream, p);
 }

@@ -130,8 +130,8 @@ int attn_plan(int64_t B, int64_t T, int64_t heads, int64_t heads_kv, int64_t D, 
     const int64_t rows = max_q_len * group, max_units = up(max_blocks * block_size, 64);
     p.width = (int32_t)W;
     // The row kernel reads the cache once per row tile: 32 rows, 16 above width 128.  64 requests of 2048 tokens, 8 heads, row kernel against tile kernel: width 64:
-    // 64 rows 53 to 65 us, 128 rows 101 to 67; width 128: 32 rows 58 to 86, 48 rows 110 to 87; width 256: 16 rows 108 to 171, 24 rows 200 to 172.
-    // (One request of 16384: 17.5 to 22.6 and 20.4 to 23.9; 24 to 31 and 26 to 31; 29 to 35 and 35 to 34.)
+    // 64 rows 52 to 50 us, 80 rows 74 to 65 (16 requests: 21.6 to 24.5, 28.3 to 29.8); width 128: 32 rows 58 to 67, 48 rows 109 to 69; width 256: 16 rows 109 to
+    // 171, 24 rows 201 to 173.
     p.tile = rows > (W == 64 ? 64 : W == 128 ? 32 : 16);
     p.min_units = 4;
     if (!p.tile) {
@@ -154,7 +154,9 @@ int attn_plan(int64_t B, int64_t T, int64_t heads, int64_t heads_kv, int64_t D, 
         p.ws_ml = slots * 16 * p.nr * W * 4;
         p.ws_prefix = p.ws_ml + slots * 16 * p.nr * 8;
     } else {
-        p.nr = W <= 128 ? 2 : 1;
+        // 128 rows per workgroup, or 64 where no request has more: 64 requests of 2048 tokens, width 128: 64 rows 72 us (with 128: 87), 80 rows 129 (88); width 256:
+        // 178 (267), 330 (269); four prompts of 2048 over 8192, width 256: 545 TFLOP/s with 64, 579 with 128
+        p.nr = rows > 64 ? 2 : 1;
         const int64_t rows_wg = 64 * p.nr, bound = T * group / rows_wg + B;
         int64_t tiles = up(T * group, rows_wg);
         if (tiles < B) tiles = B;                 // (a request with tokens has a tile of its own)
