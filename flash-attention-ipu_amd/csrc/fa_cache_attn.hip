@@ -132,59 +132,68 @@ __device__ __forceinline__ Request request_of(const CacheAttnParams& p, int b) {
     return r;
 }
 
-// Every workgroup finds its place by itself: `items(b)` summed over the requests (each thread a stretch of them), `want(total)` names the item to
-// find, and the stretch that holds it is walked.  prefix (or null) receives the sums.
 __device__ __forceinline__ long long uniform(long long x) {
     const unsigned lo = (unsigned)__builtin_amdgcn_readfirstlane((int)x), hi = (unsigned)__builtin_amdgcn_readfirstlane((int)(x >> 32));
     return (long long)((unsigned long long)hi << 32 | lo);
 }
+__device__ __forceinline__ long long lane_value(long long x, int lane) {
+    const unsigned lo = (unsigned)__builtin_amdgcn_readlane((int)x, lane), hi = (unsigned)__builtin_amdgcn_readlane((int)(x >> 32), lane);
+    return (long long)((unsigned long long)hi << 32 | lo);
+}
+template <int CTRL, int ROWS>
+__device__ __forceinline__ long long sum_step(long long x) {
+    const unsigned lo = (unsigned)__builtin_amdgcn_update_dpp(0, (int)x, CTRL, ROWS, 0xf, false), hi = (unsigned)__builtin_amdgcn_update_dpp(0, (int)(x >> 32), CTRL, ROWS, 0xf, false);
+    return x + (long long)((unsigned long long)hi << 32 | lo);
+}
+// Every wave finds its place by itself, without a barrier: `items` summed over the requests (each lane a stretch of them), `want(total)` names the item to
+// find, and the stretch that holds it is walked.  prefix (or null) receives the sums.  The request comes with it: a small call is a chain of loads.
 struct Place {
+    Request rq;
     int b;
     long long off, total;
 };
-template <int NT, typename Items, typename Want>
-__device__ __forceinline__ Place find_place(int B, Items items, Want want, long long* prefix) {
-    __shared__ long long sums[NT / 64 + 1];
-    __shared__ Place found;
-    const int tid = (int)threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int per = (B + NT - 1) / NT, from = min(tid * per, B), to = min(from + per, B);
+template <typename Items, typename Want>
+__device__ __forceinline__ Place find_place(const CacheAttnParams& p, Items items, Want want, long long* prefix) {
+    const int lane = (int)threadIdx.x & 63, per = (p.B + 63) >> 6, from = min(lane * per, p.B), to = min(from + per, p.B);
+    Place f{};
     long long mine = 0;
-    for (int b = from; b < to; ++b) mine += items(b);
+    for (int b = from; b < to; ++b) {
+        f.rq = request_of(p, b);
+        mine += items(f.rq);
+    }
     long long incl = mine;
-    for (int d = 1; d < 64; d *= 2) {
-        const long long y = __shfl_up(incl, d);
-        if (lane >= d) incl += y;
-    }
-    if (lane == 63) sums[wave] = incl;
-    __syncthreads();
-    long long before = incl - mine, total = 0;
-    for (int w = 0; w < NT / 64; ++w) {
-        if (w < wave) before += sums[w];
-        total += sums[w];
-    }
-    total = uniform(total);
-    const long long x = want(total);
-    if (x >= before && x < before + mine) {
-        long long at = before;
-        int b = from;
-        for (;; ++b) {
-            const long long n = items(b);
-            if (x < at + n) break;
-            at += n;
+    incl = sum_step<0x111, 0xf>(incl);      // row_shr 1, 2, 4, 8; then the rows' last lanes onto the rows behind them
+    incl = sum_step<0x112, 0xf>(incl);
+    incl = sum_step<0x114, 0xf>(incl);
+    incl = sum_step<0x118, 0xf>(incl);
+    incl = sum_step<0x142, 0xa>(incl);
+    incl = sum_step<0x143, 0xc>(incl);
+    const long long before = incl - mine;
+    f.total = lane_value(incl, 63);
+    const long long x = want(f.total);
+    const bool here = x >= before && x < incl;
+    f.b = from;
+    f.off = x - before;
+    if (here && per > 1)
+        for (;; ++f.b) {
+            f.rq = request_of(p, f.b);
+            const long long n = items(f.rq);
+            if (f.off < n) break;
+            f.off -= n;
         }
-        found.b = b;
-        found.off = x - at;
-    }
     if (prefix) {
         long long at = before;
-        for (int b = from; b < to; ++b) { prefix[b] = at; at += items(b); }
-        if (tid == 0) prefix[B] = total;
+        for (int b = from; b < to; ++b) { prefix[b] = at; at += items(request_of(p, b)); }
+        if (lane == 0) prefix[p.B] = f.total;
     }
-    __syncthreads();
-    Place f;
-    f.b = __builtin_amdgcn_readfirstlane(found.b);
-    f.off = uniform(found.off);
-    f.total = total;
+    const unsigned long long who = __ballot(here);
+    const int lead = who ? (int)__builtin_ctzll(who) : 0;      // (no lane: the item lies behind the last one, and the caller goes home)
+    f.b = __builtin_amdgcn_readlane(f.b, lead);
+    f.off = lane_value(f.off, lead);
+    f.rq.first = __builtin_amdgcn_readlane(f.rq.first, lead);
+    f.rq.n = __builtin_amdgcn_readlane(f.rq.n, lead);
+    f.rq.len = __builtin_amdgcn_readlane(f.rq.len, lead);
+    f.rq.units = __builtin_amdgcn_readlane(f.rq.units, lead);
     return f;
 }
 
@@ -518,21 +527,25 @@ __global__ __launch_bounds__(256, 2) void cache_rows_kernel(CacheAttnParams p) {
     const int lane = (int)threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
     const int lg = lane >> 4, wk = lane & 15;
     long long range = 1, start = 0;
-    const Place at = find_place<256>(p.B, [&](int b) { return row_items(p, request_of(p, b), ROWS); },
-                                     [&](long long total) { range = range_of(p, total); start = range * (long long)blockIdx.x; return start; },
-                                     blockIdx.x == 0 ? p.ws_prefix : nullptr);
+    const Place at = find_place(p, [&](const Request& r) { return row_items(p, r, ROWS); },
+                                [&](long long total) { range = range_of(p, total); start = range * (long long)blockIdx.x; return start; },
+                                blockIdx.x == 0 && wave == 0 ? p.ws_prefix : nullptr);
     if (start >= at.total) return;
     const long long end = start + range < at.total ? start + range : at.total;
     int b = at.b;
     long long off = at.off, cur = start;
     const unsigned key_off = UnitAt<SMALL>::key_lane(W, lane), value_off = UnitAt<SMALL>::value_lane(p.shift, lane);
     State st;
+    Request rq = at.rq;
     while (cur < end) {
-        const Request rq = request_of(p, b);
         const int tiles = (rq.n * p.group + ROWS - 1) / ROWS;
         const int per = p.whole ? 1 : rq.units;            // items of a row tile
         const long long items = (long long)tiles * p.Hkv * per;
-        if (off >= items) { ++b; off = 0; continue; }      // (the next request with rows; there is one, cur < end)
+        if (off >= items) {                                // (the next request with rows; there is one, cur < end)
+            rq = request_of(p, ++b);
+            off = 0;
+            continue;
+        }
         const int ht = (int)(off / per), u0 = (int)(off - (long long)ht * per);
         const int h = ht / tiles, row0 = (ht - h * tiles) * ROWS;
         const int u1 = p.whole || u0 + (end - cur) >= rq.units ? rq.units : (int)(u0 + (end - cur));
@@ -705,8 +718,8 @@ __global__ __launch_bounds__(256, W > 128 ? 1 : 2) void cache_tile_kernel(CacheA
     // or is a multiple of it; late tiles (the long ones of a prompt) first
     const int idx = (int)blockIdx.x, h = idx % p.Hkv, rest = idx / p.Hkv, part = rest % p.splits, order = rest / p.splits;
     long long tile = 0;
-    const Place at = find_place<256>(p.B, [&](int b) { return (long long)((request_of(p, b).n * p.group + ROWS - 1) / ROWS); },
-                                     [&](long long total) { tile = total - 1 - order; return tile; }, blockIdx.x == 0 ? p.ws_prefix : nullptr);
+    const Place at = find_place(p, [&](const Request& r) { return (long long)((r.n * p.group + ROWS - 1) / ROWS); },
+                                [&](long long total) { tile = total - 1 - order; return tile; }, blockIdx.x == 0 && wave == 0 ? p.ws_prefix : nullptr);
     if (order >= at.total || tile >= p.max_tiles) return;      // (more tiles than tokens allow: cu_q is not ascending)
     const Request rq = request_of(p, at.b);
     const int row0 = (int)at.off * ROWS;
@@ -804,7 +817,7 @@ __global__ __launch_bounds__(256, W > 128 ? 1 : 2) void cache_tile_kernel(CacheA
         st.weights(s[A], w, here.kf, here.vs);
         mix<4 * NC * NR, 4 * NC, 8, 2>();
         __builtin_amdgcn_sched_barrier(0);
-        if (SMALL) after.find(p, table, rq.len, min(u + 2, u1 - 1), h, W, lane);     // (addresses of every lane: formed where registers are free)
+        if (SMALL) after.find(p, table, rq.len, min(u + 2, u1 - 1), h, W, fresh_lane(lane));     // (addresses of every lane: formed where registers are free)
         load_keys(after);                                           // (here, where the scores of u have left their registers)
         load_values(next);
         float top[NR];
