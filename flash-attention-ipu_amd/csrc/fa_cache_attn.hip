@@ -518,9 +518,10 @@ __global__ __launch_bounds__(256, 2) void cache_rows_kernel(CacheAttnParams p) {
     using State = RowState<T, W, NR>;
     constexpr int ND = State::ND, NK = W / 64, ROWS = 16 * NR;
     // the next unit's codes are fetched under this one's arithmetic where the registers hold them beside O; else a unit's value columns are
-    // taken in parts
+    // taken in parts, as large as the registers hold (width 256, 64 requests of 4096: quarters 172 us, eighths 189; 32 rows of width 128 over 2048: halves 52.5,
+    // quarters 58)
     constexpr bool AHEAD = W * NR <= 128;
-    constexpr int VN = AHEAD ? ND : W > 192 ? ND / 8 : W * NR > 192 ? ND / 4 : ND / 2;
+    constexpr int VN = AHEAD ? ND : W > 192 ? (SMALL ? ND / 8 : ND / 4) : ND / 2;
     __shared__ __align__(8) unsigned short nan_keys[4][4 * W];     // [wave][column][16-key group]
     __shared__ f32x4 join_o[2][NR * ND * 64];
     __shared__ float join_m[4][ROWS], join_l[4][ROWS];

@@ -130,19 +130,19 @@ int attn_plan(int64_t B, int64_t T, int64_t heads, int64_t heads_kv, int64_t D, 
     const int64_t rows = max_q_len * group, max_units = up(max_blocks * block_size, 64);
     p.width = (int32_t)W;
     // The row kernel reads the cache once per row tile: 32 rows, 16 above width 128.  64 requests of 2048 tokens, 8 heads, row kernel against tile kernel: width 64:
-    // 64 rows 52 to 50 us, 80 rows 74 to 65 (16 requests: 21.6 to 24.5, 28.3 to 29.8); width 128: 32 rows 58 to 67, 48 rows 109 to 69; width 256: 16 rows 109 to
-    // 171, 24 rows 201 to 173.
+    // 64 rows 52 to 49 us, 80 rows 74 to 64 (16 requests: 21.5 to 23.6, 28.4 to 29.5); width 128: 32 rows 56 to 67, 48 rows 103 to 70; width 256: 16 rows 100 to
+    // 170, 24 rows 184 to 171.
     p.tile = rows > (W == 64 ? 64 : W == 128 ? 32 : 16);
     p.min_units = 4;
     if (!p.tile) {
-        // 32 rows in one pass or 16 in each of two (64 requests of 2048: 20 rows of width 128 57 to 88 us); for up to 16 rows the smaller tile (49 to 55)
+        // 32 rows in one pass or 16 in each of two (64 requests of 2048: 20 rows of width 64 28 to 44 us); for up to 16 rows the smaller tile (25.8 to 27.8)
         p.nr = rows > 16 ? 2 : 1;
         p.max_tiles = (int32_t)up(rows, 16 * p.nr);
         // two resident workgroups per compute unit (64 requests of 4096, width 128: 86.4 us; one 89, three 104, four 97; width 64: 45.6, 49.1, 52.3, 49.3);
-        // at least four units for each, a round of its waves (one request of 8192: 13.9 us; one unit 14.5, eight 15.3)
+        // at least four units for each, a round of its waves (one request of 8192: 13.1 us; one unit 13.7, eight 14.4)
         int64_t grid = 2 * kCus;
         // short caches: four waves are through a row's units in a few rounds, which is less than a second launch takes (one request of 1024 tokens, whole against
-        // cut: width 64 8.5 to 10.6 us, 128 11.5 to 12.1, 256 21 to 16.9; of 512: 16.3 to 17.5 there; of 2048: 12.1 to 10.6, 17 to 12.6)
+        // cut: width 64 8.5 to 10.5 us, 128 11.5 to 12.3, 256 18.2 to 15.0; of 512: 14.2 to 14.9 there; of 2048: 12.1 to 10.6, 17 to 12.6)
         p.whole = max_units <= (W <= 128 ? 16 : 8);
         if (p.whole) p.min_units = 1;
         const int64_t most = p.whole ? B * heads_kv * p.max_tiles : up(B * heads_kv * p.max_tiles * max_units, p.min_units);
