@@ -114,7 +114,7 @@ def _bwd_impl(q, k, dq_out, dk_out, q_weight, k_weight, table, positions, eps, i
     ws, nbytes = None, 0
     if need_q_weight or need_k_weight:
         nbytes = call.workspace
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
+        ws = table.new_empty(nbytes // 4)
     stream, prev = _native.stream_of(q.device)
     try:
         rc = _native._LIB.fa_qk_norm_rope_bwd(q.data_ptr(), k.data_ptr(), dq_out.data_ptr(), dk_out.data_ptr(), dq.data_ptr(), dk.data_ptr(),
