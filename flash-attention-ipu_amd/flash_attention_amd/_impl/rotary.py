@@ -238,6 +238,9 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: Optional[torch.Tens
                 A position that the table lacks gives NaN.
     interleaved False: columns (i, i + rotary dim / 2) are a pair; True: (2 i, 2 i + 1)
     returns     (q, k) normed and rotated, in the operands' layout
+
+    A training step can be captured.  As everywhere in torch, a captured backward() must not meet an eager graph of the same leaves that is still alive: free its
+    outputs first, or take the gradients with torch.autograd.grad.
     """
     if not 0.0 <= eps < float("inf"):
         raise ValueError(f"qk_norm_rope: eps must be finite and >= 0 (got {eps})")

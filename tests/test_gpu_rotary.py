@@ -244,6 +244,28 @@ def test_partial_gradients_and_double_backward(rot):
         g.sum().backward()
 
 
+def test_broadcast_operands(rot):
+    """operands, positions and incoming gradients with strides of zero, one weight for both sides"""
+    g = torch.Generator().manual_seed(12)
+    B, H, Hk, L, D = 3, 4, 2, 37, 64
+    table = rot.rotary_table(L + 9, D, device=DEV)
+    q0, k0 = (torch.randn(*s, generator=g).to(DEV).requires_grad_() for s in ((1, H, L, D), (B, 1, L, D)))
+    w = (1 + 0.2 * torch.randn(D, generator=g)).to(DEV).requires_grad_()
+    pos = torch.randint(0, L + 9, (1, L), generator=g)
+    q, k = q0.expand(B, H, L, D), k0.expand(B, Hk, L, D)
+    o = rot.qk_norm_rope(q, k, w, w, table, pos.to(DEV).expand(B, L))
+    gq, gk, gw = torch.autograd.grad([t.sum() for t in o], (q0, k0, w))
+    dws = []
+    for x, h, y, got, dims in ((q, H, o[0], gq, 0), (k, Hk, o[1], gk, 1)):
+        full = pos.repeat(B, 1).reshape(-1).repeat_interleave(h)
+        out, mag, dx, dxm, dw, dwm = reference(rows(x), w.detach().cpu().double(), table.cpu(), full, 1e-6, False, torch.ones(B * L * h, D, dtype=torch.float64))
+        close(rows(y), out, mag, torch.float32, 24)
+        back = lambda t: t.reshape(B, L, h, D).transpose(1, 2).sum(dims, keepdim=True)  # noqa: E731
+        close(rows(got), rows(back(dx)), rows(back(dxm)), torch.float32, 64 + 3)
+        dws.append((dw, dwm))
+    close(gw.cpu().double(), dws[0][0] + dws[1][0], dws[0][1] + dws[1][1], torch.float32, B * L * H + 65)
+
+
 def test_only_one_output_used(rot):
     table = rot.rotary_table(8, 64, device=DEV)
     q, k = torch.randn(5, 3, 64, device=DEV, requires_grad=True), torch.randn(5, 1, 64, device=DEV, requires_grad=True)
