@@ -27,6 +27,14 @@ def plain_norm_rope(q, k, q_weight, k_weight, table, positions=None, eps=1e-6):
     return one(q, q_weight), one(k, k_weight)
 
 
+def attention(q, k, v, attn_mask=None, dropout_p=0.0, is_causal=False, enable_gqa=False):
+    """causal attention written out in 32 bits, whatever serves the call elsewhere (an override that another test installed takes some lengths only)"""
+    assert q.dtype == torch.float32 and is_causal
+    k, v = (t.repeat_interleave(q.shape[1] // t.shape[1], 1) for t in (k, v))
+    s = (q @ k.transpose(-1, -2)) * q.shape[-1] ** -0.5
+    return s.masked_fill(torch.ones(s.shape[-2:], device=s.device, dtype=torch.bool).triu(1), float("-inf")).softmax(-1) @ v
+
+
 @pytest.mark.parametrize("n_kv_head", [4, 2, 1])
 def test_gradients_of_a_step(n_kv_head, monkeypatch):
     torch.manual_seed(3)
@@ -43,12 +51,6 @@ def test_gradients_of_a_step(n_kv_head, monkeypatch):
         loss.backward()
         return loss.item(), {n: p.grad.clone() for n, p in net.named_parameters()}
 
-    def attention(q, k, v, attn_mask=None, dropout_p=0.0, is_causal=False, enable_gqa=False):
-        # (written out: two passes of one attention in 32 bits, whatever serves the call elsewhere)
-        k, v = (t.repeat_interleave(q.shape[1] // t.shape[1], 1) for t in (k, v))
-        s = (q @ k.transpose(-1, -2)) * q.shape[-1] ** -0.5
-        return s.masked_fill(torch.ones(s.shape[-2:], device=s.device, dtype=torch.bool).triu(1), float("-inf")).softmax(-1) @ v
-
     monkeypatch.setattr(F, "scaled_dot_product_attention", attention)
     loss, grads = step()
     monkeypatch.setattr(demo_model, "qk_norm_rope", plain_norm_rope)
@@ -61,7 +63,8 @@ def test_gradients_of_a_step(n_kv_head, monkeypatch):
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("n_kv_head,block_size", [(4, 64), (1, 16)])
-def test_steps_over_the_cache(n_kv_head, block_size, dtype):
+def test_steps_over_the_cache(n_kv_head, block_size, dtype, monkeypatch):
+    monkeypatch.setattr(F, "scaled_dot_product_attention", attention)
     torch.manual_seed(4)
     net = gpt2_init_(TinyGPT(vocab=97, block=160, n_layer=2, n_head=4, n_embd=256, n_kv_head=n_kv_head, rotary=True), std=0.05).cuda().eval()
     lens = [1, 70, 128, 33]
