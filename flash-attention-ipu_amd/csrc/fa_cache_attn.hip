@@ -12,7 +12,7 @@
 //   * the value cache is token-inner, so the matching A operand (column d, those sixteen keys) is one 16-byte load, as is a key row's share.
 // e4m3 -> 16-bit is exact, one instruction per two values.  Scales cost no instruction per score: scale_k and the softmax scale are the factor
 // of the exponent's fma, and the weight that meets the codes of V is P' = P scale_v / ref = 2^(s kf - (max - log2(scale_v / ref))), rounded once to
-// the operand type; the sum of the weights takes a lane's sum of P' times ref / scale_v, once per unit.  ref: 1 for bf16, whose exponents reach as
+// the operand type; the sum of the weights takes a lane's sum of P' (bf16: rounded) times ref / scale_v, once per unit.  ref: 1 for bf16, whose exponents reach as
 // far as 32-bit ones; for f16 a reference that follows the scales and keeps the weights between its subnormals and its largest value.
 // Maximum, sum and O are 32-bit.
 //
@@ -25,7 +25,7 @@
 //                64 requests of 4600 tokens on average, 8 heads of 128: 105 us = 5.7 TB/s, every code read once, and 5 us for the join.
 //   tile kernel  128 rows per workgroup, 64 where no request has more (prompts): bound by the matrix pipe.  Four waves share a unit's operands,
 //                converted once into LDS in the very order in which the lanes read them.  Grids too small for the chip cut every tile's
-//                key range into `splits` parts.  Four prompts of 2048 over 8192 tokens, 32 / 8 heads: 1020 TFLOP/s at width 128, 680 at 64, 580 at 256
+//                key range into `splits` parts.  Four prompts of 2048 over 8192 tokens, 32 / 8 heads: bf16 1015 TFLOP/s at width 128, 690 at 64, 630 at 256 (f16 980, 655, 576)
 //                (matrix pipe 39 % busy, vector issue 41 %, LDS 51 %).
 // Stale codes behind a request's end are cleared before they meet a zero weight (0 * NaN), and a NaN code that only some rows of a unit may
 // see reaches those rows alone.
@@ -339,10 +339,18 @@ struct RowState {
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     e[i] = fast_exp2(__builtin_fmaf(s[r][t][i], kf, base));
-                    sum[i & 1] += e[i];
+                    if constexpr (kRef) sum[i & 1] += e[i];
                 }
                 u[2 * t] = pack2<T>(e[0], e[1]);
                 u[2 * t + 1] = pack2<T>(e[2], e[3]);
+                // bf16: one instruction adds two rounded weights (width 256, prompts of 2048 over 8192: 4190 -> 3900 us, width 192 3275 -> 3105, width 128 1 % or less).
+                // f16 weights that meet small values round to zero and still count in the sum: they are added before they are rounded.
+                if constexpr (!kRef) {
+                    typedef __bf16 vec2 __attribute__((ext_vector_type(2)));
+                    const vec2 one = {(__bf16)1.0f, (__bf16)1.0f};
+                    sum[0] = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(vec2, u[2 * t]), one, sum[0], false);
+                    sum[1] = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(vec2, u[2 * t + 1]), one, sum[1], false);
+                }
             }
             l[r] = __builtin_fmaf(sum[0] + sum[1], back, l[r]);
             asm volatile("" : "+v"(l[r]));            // (here: moved behind the products, the sum would keep every weight in a register)
@@ -716,11 +724,15 @@ __global__ __launch_bounds__(256, W > 128 ? 1 : 2) void cache_tile_kernel(CacheA
     const int lane = (int)threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
     const int lg = lane >> 4, wk = lane & 15;
     // block -> (head, part, tile): the head is the fastest, so that the tiles that share codes run on one XCD where the head count divides 8
-    // or is a multiple of it; late tiles (the long ones of a prompt) first
+    // or is a multiple of it; late tiles (the long ones of a prompt) first.  Where two workgroups per compute unit take all of them, the second ones come in the
+    // other order: the longest beside the shortest (one prompt of 2048, 32 / 8 heads of 128:
+    // 74.5 -> 70.6 us; eight of 256 over 1024: 53.3 -> 51.6).  `half`: tiles of a head that one workgroup per compute unit takes
     const int idx = (int)blockIdx.x, h = idx % p.Hkv, rest = idx / p.Hkv, part = rest % p.splits, order = rest / p.splits;
+    const int half = W <= 128 ? 256 / (p.Hkv * p.splits) : 0x3fffffff;
     long long tile = 0;
     const Place at = find_place(p, [&](const Request& r) { return (long long)((r.n * p.group + ROWS - 1) / ROWS); },
-                                [&](long long total) { tile = total - 1 - order; return tile; }, blockIdx.x == 0 && wave == 0 ? p.ws_prefix : nullptr);
+                                [&](long long total) { tile = order >= half && total <= 2 * half ? order - half : total - 1 - order; return tile; },
+                                blockIdx.x == 0 && wave == 0 ? p.ws_prefix : nullptr);
     if (order >= at.total || tile >= p.max_tiles) return;      // (more tiles than tokens allow: cu_q is not ascending)
     const Request rq = request_of(p, at.b);
     const int row0 = (int)at.off * ROWS;

@@ -222,11 +222,12 @@ def random_cache(kv, g, N, H, P, D):
 
 
 def tolerance(dtype, out, mag, vmax, keys):
-    """u: half a step.  The output is rounded once, every weight once (against the weights' sum, which is not): u |o| + u sum p |v|.  32-bit products, maximum and
-    exponentials: a score of magnitude s is off by some s 2^-22 and its weight by as much; 2^-12 sum p |v| covers |s| up to 2^10.  A weight below the smallest
-    normal half is off by at most 2^-25 (the sum of the weights is at least 1)."""
+    """u: half a step.  The output is rounded once, every weight once: u |o| + u sum p |v|.  Half weights are added up before they are rounded, bf16 ones after:
+    sum w (1 + d) v / sum w (1 + d) with |d| <= u is off by at most u sum p |v - o| <= u (sum p |v| + |o|).  32-bit products, maximum and exponentials: a score of
+    magnitude s is off by some s 2^-22 and its weight by as much; 2^-12 sum p |v| covers |s| up to 2^10.  A weight below the smallest normal half is off by at most
+    2^-25 (the sum of the weights is at least 1)."""
     u = torch.finfo(dtype).eps / 2
-    return u * out.abs() + (u + 2.0 ** -12) * mag + (keys * 2.0 ** -25 * vmax if dtype == torch.float16 else 1e-30)
+    return (u if dtype == torch.float16 else 2 * u) * out.abs() + (u + 2.0 ** -12) * mag + (keys * 2.0 ** -25 * vmax if dtype == torch.float16 else 1e-30)
 
 
 def check_attention(kv, held, new, Hkv, group, D, P, dtype, seed=0, max_q_len=None, bad=(), poke=None, pad=0, cache=None):
