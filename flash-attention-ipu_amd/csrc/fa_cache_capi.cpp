@@ -296,9 +296,9 @@ int fa_cache_append(const void* k, const void* v, const int32_t* slots, void* k_
     }
     p.T = (int32_t)num_tokens; p.H = (int32_t)heads_kv; p.D = (int32_t)D; p.W = (int32_t)W; p.shift = block_shift(block_size);
     p.limit = num_blocks * block_size;
-    // tokens per workgroup: about 1024 workgroups in all, which the chip holds at once.  Steps of single tokens spread over the chip (64 tokens of 8 heads of 128: 5.5 us
-    // with 4, 15 with 16, 50 with 64), prompts do not pay for workgroups in which no run begins (16384 tokens: 204 us with 4, 59 with 16, 27 with 64;
-    // 2048: 30, 11.8 and 8.5).
+    // tokens per workgroup: about 1024 workgroups in all, which the chip holds at once.  Steps of single tokens spread over the chip (64 tokens of 8 heads of 128: 5.4 us
+    // with 4, 12 with 16, 40 with 64), prompts do not pay for workgroups in which no run begins (16384 tokens: 82 us with 4, 51 with 16, 22 with 64;
+    // 2048: 13.6, 8.8 and 8.0, with 32 6.2).
     int window = 4;
     while (window < 64 && up(num_tokens, window) * 2 * heads_kv > 1024) window *= 2;
     p.window = window;

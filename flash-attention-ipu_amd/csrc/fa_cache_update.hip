@@ -290,7 +290,8 @@ __device__ __forceinline__ void transpose4(unsigned (&r)[4]) {
 
 // One run: tokens t0 .. t0 + n - 1 into positions off .. off + n - 1 of a block.  NT = 64 (a wave) or 256 (the workgroup).
 // HOLD: items per thread that stay in registers between the maximum and the codes: one where a whole block is one item per thread of a workgroup
-// (16384 tokens in blocks of 64, 8 heads of 128: 30.4 us, with two 32.0; of 64: 17.0 and 18.8), else two (blocks of 128: 26.3 us, with one 28.9).
+// (24 prompts of up to 2048, blocks of 64, 8 heads of 128: 30.4 us, with two 32.0; 16384 tokens, heads of 64: 17.0 and 18.8), else two (16384 tokens, blocks of 128:
+// 26.3 us, with one 28.9).
 template <typename T, int W, int HOLD, bool KEYS, int NT>
 __device__ __forceinline__ void append_run(const AppendParams& p, int t0, int n, int64_t block, int off, int head, unsigned* shared_max) {
     constexpr int S = KEYS ? 0 : 1, WC = W / 8;                           // column chunks of a row
@@ -459,7 +460,7 @@ __global__ __launch_bounds__(256) void cache_append_kernel(AppendParams p) {
             n += more;
             if (more == 64) n += ones(on2);
         }
-        const bool together = few && n >= 16;     // (of several runs, or for a short one, a wave each: 512 tokens of one request 6.7 us, 10.5 without)
+        const bool together = few && n >= 16;     // (of several runs, or for a short one, a wave each: 512 tokens of one request 6.1 us, 10.5 without)
         if (!together && (r & 3) != wave) continue;
         const int t0 = t_first + i, slot = __builtin_amdgcn_readfirstlane(p.slots[t0]);
         const int64_t block = slot >> p.shift;
