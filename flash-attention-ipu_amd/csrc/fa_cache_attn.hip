@@ -475,8 +475,19 @@ struct UnitAt {
             top = vs;
         } else {
             const int kk = first + 16 * (wk >> 2), vk = first + 16 * lg;
-            const int kid = kk < len ? block_at(p, table, kk >> p.shift) : -1;
-            const int vid = vk < len ? block_at(p, table, vk >> p.shift) : -1;
+            // The blocks of the unit's sixteen-key pieces are uniform: scalar loads.  (As the lanes' own loads they would come behind the codes in flight, and every
+            // unit would wait for them: 64 requests of 4096, blocks of 16: width 64 54 us, so 48; width 128 99 and 94.  The scales as scalar loads too: 63 and 102.)
+            int ids[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int key = first + 16 * j, index = key >> p.shift, id = constant(table + (index < p.width ? index : p.width - 1));
+                ids[j] = key < len && index < p.width && (unsigned)id < (unsigned)p.num_blocks ? id : -1;
+            }
+            const auto pick = [&](int j) {
+                const int a = j & 1 ? ids[1] : ids[0], b = j & 1 ? ids[3] : ids[2];
+                return j & 2 ? b : a;
+            };
+            const int kid = pick(wk >> 2), vid = pick(lg);
             dead = vid < 0;
             none = !__any(!dead);
             const long long kb = kid < 0 ? 0 : kid, vb = vid < 0 ? 0 : vid;
