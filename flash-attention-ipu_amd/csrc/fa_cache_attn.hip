@@ -11,10 +11,11 @@
 //     CONSECUTIVE keys 16 (lane >> 4) .. + 15, which is what the B operand of the second product wants of that lane (two products of 32 keys);
 //   * the value cache is token-inner, so the matching A operand (column d, those sixteen keys) is one 16-byte load, as is a key row's share.
 // e4m3 -> 16-bit is exact, one instruction per two values.  Scales cost no instruction per score: scale_k and the softmax scale are the factor
-// of the exponent's fma, and the weight that meets the codes of V is P' = P scale_v / ref = 2^(s kf - (max - log2(scale_v / ref))), rounded once to
-// the operand type; the sum of the weights takes a lane's sum of P' (bf16: rounded) times ref / scale_v, once per unit.  ref: 1 for bf16, whose exponents reach as
-// far as 32-bit ones; for f16 a reference that follows the scales and keeps the weights between its subnormals and its largest value.
-// Maximum, sum and O are 32-bit.
+// of the exponent's fma, and the weight that meets the codes of V is P' = P scale_v = 2^(s kf + log2(scale_v) - max), rounded once to the operand type; the
+// sum of the weights takes a lane's sum of P' (bf16: rounded) over scale_v, once per unit.  `max` is the row's largest score for bf16, whose exponents reach as
+// far as 32-bit ones.  f16 weights have thirty binades and ten of subnormals, and a row's scales may differ by more: its `max` is the largest s kf + log2(scale_v)
+// of the keys that the row sees, less kLift, so that the largest P' stays near the type's top and what vanishes is 2^-32 of the row's own largest term,
+// whatever the scales of blocks are that it does not see or gives no weight.  Maximum, sum and O are 32-bit.
 //
 // Two kernels:
 //   row kernel   few rows per key/value head (a decoding step): bound by the cache's bytes.  Codes go from memory straight into
@@ -25,7 +26,7 @@
 //                64 requests of 4600 tokens on average, 8 heads of 128: 105 us = 5.7 TB/s, every code read once, and 5 us for the join.
 //   tile kernel  128 rows per workgroup, 64 where no request has more (prompts): bound by the matrix pipe.  Four waves share a unit's operands,
 //                converted once into LDS in the very order in which the lanes read them.  Grids too small for the chip cut every tile's
-//                key range into `splits` parts.  Four prompts of 2048 over 8192 tokens, 32 / 8 heads: bf16 1015 TFLOP/s at width 128, 690 at 64, 630 at 256 (f16 980, 655, 576)
+//                key range into `splits` parts.  Four prompts of 2048 over 8192 tokens, 32 / 8 heads: bf16 1014 TFLOP/s at width 128, 695 at 64, 638 at 256 (f16 1004, 682, 590)
 //                (matrix pipe 39 % busy, vector issue 41 %, LDS 51 %).
 // Stale codes behind a request's end are cleared before they meet a zero weight (0 * NaN), and a NaN code that only some rows of a unit may
 // see reaches those rows alone.
@@ -208,19 +209,17 @@ struct RowState {
     using vec8 = typename Elt<T>::vec8;
     vec8 q[NR][NC];
     f32x4 o[NR][ND];
-    float ref;                                           // f16: O is in units of this value scale (uniform; 0 = none yet), and the largest it was
-    float ref_max;
     float m[NR], l[NR];
     int limit[NR];                                       // keys that the lane's row sees
     int limit_min, limit_max;                            // over the wave's rows (uniform)
     using NanBits = typename std::conditional<W <= 128, unsigned, unsigned long long>::type;
     NanBits nan[NR];                                     // bit 4 d + i: o[r][d][i] saw a NaN value (note_nan)
 
-    static constexpr bool kRef = Elt<T>::is_f16;
+    // f16: with weights up to 2^(kSlack + kLift) = 2^15 the largest stay inside the type
+    static constexpr bool kHalf = Elt<T>::is_f16;
+    static constexpr float kSlack = 8.f, kLift = kHalf ? 7.f : 0.f;
 
     __device__ __forceinline__ void clear() {
-        ref = kRef ? 0.f : 1.f;
-        ref_max = ref;
 #pragma unroll
         for (int r = 0; r < NR; ++r) {
             m[r] = -INFINITY;
@@ -280,8 +279,12 @@ struct RowState {
                 for (int i = 0; i < 4; ++i) s[r][t][i] = 4 * t + i < see ? s[r][t][i] : -INFINITY;
         }
     }
-    // every row's largest score of the unit, in powers of two.  kf: scale_k times the softmax scale
-    __device__ __forceinline__ void peak(const f32x4 (&s)[NR][4], float kf, float (&top)[NR]) const {
+    // The value scale that the weights carry.  f16: one below 2^-64 counts as 2^-64 (448 times that is far below half of the smallest f16 output), so that P' of a block
+    // of zeros beside large values does not leave 32-bit floats, and its weights stay in the sum.
+    static __device__ __forceinline__ float carried(float vs) { return kHalf ? __builtin_fmaxf(vs, 0x1p-64f) : vs; }
+    // every row's largest exponent of the unit: score, f16 with the value scale.  kf: scale_k times the softmax scale; vs: the lane's value scale
+    __device__ __forceinline__ void peak(const f32x4 (&s)[NR][4], float kf, float vs, float (&top)[NR]) const {
+        const float lift = kHalf ? __builtin_amdgcn_logf(carried(vs)) : 0.f;
 #pragma unroll
         for (int r = 0; r < NR; ++r) {
             float x = -INFINITY;
@@ -289,12 +292,11 @@ struct RowState {
             for (int t = 0; t < 4; ++t)
 #pragma unroll
                 for (int i = 0; i < 4; i += 2) x = __builtin_fmaxf(__builtin_fmaxf(x, s[r][t][i]), s[r][t][i + 1]);
-            top[r] = rows_max(x * kf);
+            top[r] = rows_max(kHalf ? __builtin_fmaf(x, kf, lift) : x * kf);
         }
     }
-    // the reference maximum goes up where a score would leave 2^kSlack above it (weights up to 2^kSlack round as well as weights up to 1); most units do not
+    // the reference maximum goes up where an exponent would leave 2^kSlack above it (weights up to 2^kSlack round as well as weights up to 1); most units do not
     // pay for the rescale
-    static constexpr float kSlack = 8.f;
     __device__ __forceinline__ void raise(const float (&top)[NR]) {
 #pragma unroll
         for (int r = 0; r < NR; ++r) {
@@ -307,27 +309,10 @@ struct RowState {
             }
         }
     }
-    // f16: scale_v / ref stays in 2^-3 .. 2^7: with P up to 2^kSlack the weights stay below 2^15 and, where P is not small against its row's largest, above
-    // 2^-14.  top: the unit's largest value scale.  ref goes down to 2^-40 of the largest it was: values of scales far below that vanish beside the others, and O
-    // in units of ref stays finite
-    __device__ __forceinline__ void follow(float top) {
-        if constexpr (kRef) {
-            const float low = ref_max * 0x1p-40f;
-            if (top > ref * 128.f || (top * 8.f < ref && ref > low)) {       // (uniform)
-                const float now = __builtin_fmaxf(top * 0.125f, low), f = ref / now;
-#pragma unroll
-                for (int r = 0; r < NR; ++r)
-#pragma unroll
-                    for (int d = 0; d < ND; ++d) o[r][d] *= f;
-                ref = now;
-                ref_max = __builtin_fmaxf(ref_max, now);
-            }
-        }
-    }
     // P' of a unit, and its sum into l.  vs: the lane's value scale
     __device__ __forceinline__ void weights(const f32x4 (&s)[NR][4], vec8 (&w)[NR][2], float kf, float vs) {
-        const float shift = __builtin_amdgcn_logf(kRef ? vs * __builtin_amdgcn_rcpf(ref) : vs);
-        const float back = kRef ? ref * __builtin_amdgcn_rcpf(vs) : __builtin_amdgcn_rcpf(vs);
+        vs = carried(vs);
+        const float shift = __builtin_amdgcn_logf(vs) + kLift, back = __builtin_amdgcn_rcpf(vs);
 #pragma unroll
         for (int r = 0; r < NR; ++r) {
             const float base = shift - (m[r] == -INFINITY ? 0.f : m[r]);
@@ -339,13 +324,13 @@ struct RowState {
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     e[i] = fast_exp2(__builtin_fmaf(s[r][t][i], kf, base));
-                    if constexpr (kRef) sum[i & 1] += e[i];
+                    if constexpr (kHalf) sum[i & 1] += e[i];
                 }
                 u[2 * t] = pack2<T>(e[0], e[1]);
                 u[2 * t + 1] = pack2<T>(e[2], e[3]);
                 // bf16: one instruction adds two rounded weights (width 256, prompts of 2048 over 8192: 4190 -> 3900 us, width 192 3275 -> 3105, width 128 1 % or less).
                 // f16 weights that meet small values round to zero and still count in the sum: they are added before they are rounded.
-                if constexpr (!kRef) {
+                if constexpr (!kHalf) {
                     typedef __bf16 vec2 __attribute__((ext_vector_type(2)));
                     const vec2 one = {(__bf16)1.0f, (__bf16)1.0f};
                     sum[0] = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(vec2, u[2 * t]), one, sum[0], false);
@@ -374,16 +359,6 @@ struct RowState {
             if (FENCE && (NR * W > 128 || d % 2)) __builtin_amdgcn_sched_barrier(0);
         }
     }
-    // the segment's end: O in plain units, NaN where it was seen
-    __device__ __forceinline__ void finish() {
-        if constexpr (kRef) {
-#pragma unroll
-            for (int r = 0; r < NR; ++r)
-#pragma unroll
-                for (int d = 0; d < ND; ++d) o[r][d] *= ref;
-        }
-        put_nan();
-    }
     // A unit that some rows see only in part holds NaN values: they were taken out of the operands (take_nan) and are noted for the rows that see
     // them; keys[column]: the unit's keys with NaN in that column
     __device__ __forceinline__ void note_nan(const unsigned long long* keys, int unit, int lg) {
@@ -399,6 +374,7 @@ struct RowState {
             }
         }
     }
+    // the segment's end: NaN where it was seen
     __device__ __forceinline__ void put_nan() {
 #pragma unroll
         for (int r = 0; r < NR; ++r) {
@@ -453,7 +429,7 @@ template <bool SMALL>
 struct UnitAt {
     const uint8_t* k;
     const uint8_t* v;
-    float kf, vs, top;        // the lane's factors (softmax()), the unit's largest value scale
+    float kf, vs;             // the lane's factors: scale_k times the softmax scale, the value scale
     bool dead, none;          // the lane's sixteen keys have no block; the unit has none at all (uniform)
     bool blank;               // their values count as zeros: no block, or a scale of zero
     // (a scale of zero, or none, becomes one that makes everything vanish but leaves no 0 * inf)
@@ -472,7 +448,6 @@ struct UnitAt {
             vs = none ? 0.f : constant(p.vs + blk * p.vs_bs + h);
             blank = vs == 0.f;
             vs = factor(vs);
-            top = vs;
         } else {
             const int kk = first + 16 * (wk >> 2), vk = first + 16 * lg;
             // The blocks of the unit's sixteen-key pieces are uniform: scalar loads.  (As the lanes' own loads they would come behind the codes in flight, and every
@@ -497,7 +472,6 @@ struct UnitAt {
             vs = dead ? 0.f : constant(p.vs + vb * p.vs_bs + h);
             blank = vs == 0.f;
             vs = factor(vs);
-            top = rows_max(vs);
         }
     }
     // byte offset of key tile 0's row of this lane, and of its row of value column 0
@@ -612,9 +586,8 @@ __global__ __launch_bounds__(256, 2) void cache_rows_kernel(CacheAttnParams p) {
                 else drop_keys();
                 if (boundary || (SMALL && __any(here.dead))) st.mask(s, key0, here.dead);
                 float top[NR];
-                st.peak(s, here.kf, top);
+                st.peak(s, here.kf, here.vs, top);
                 st.raise(top);
-                st.follow(here.top);
                 st.weights(s, w, here.kf, here.vs);
                 bool nan = false;
                 const auto part = [&](auto from) {
@@ -658,7 +631,7 @@ __global__ __launch_bounds__(256, 2) void cache_rows_kernel(CacheAttnParams p) {
         }
         // the waves' parts joined, the first wave ends with the sums
         const int active = min(4, u1 - u0);
-        st.finish();
+        st.put_nan();
     float sum[NR], top[NR];
 #pragma unroll
         for (int r = 0; r < NR; ++r) { sum[r] = rows_sum(st.l[r]); top[r] = st.m[r]; }
@@ -809,7 +782,7 @@ __global__ __launch_bounds__(256, W > 128 ? 1 : 2) void cache_tile_kernel(CacheA
     // what stands between a unit's scores and its weights
     const auto prepare = [&](int u, const UnitAt<SMALL>& a, f32x4 (&x)[NR][4], float (&top)[NR]) {
         if (64 * u + 64 > st.limit_min || __any(a.dead)) st.mask(x, 64 * u + 16 * lg, a.dead);
-        st.peak(x, a.kf, top);
+        st.peak(x, a.kf, a.vs, top);
     };
     if (u0 < u1) {
         here.find(p, table, rq.len, u0, h, W, lane);
@@ -827,7 +800,6 @@ __global__ __launch_bounds__(256, W > 128 ? 1 : 2) void cache_tile_kernel(CacheA
         scores(0, s[0]);
         prepare(u0, here, s[0], top);
         st.raise(top);
-        st.follow(here.top);
     }
     __syncthreads();                                                // (unit u0's keys are read: round u0 fetches u0 + 2's over them)
     const auto round = [&](int u, auto which) {
@@ -848,14 +820,11 @@ __global__ __launch_bounds__(256, W > 128 ? 1 : 2) void cache_tile_kernel(CacheA
         if (64 * u + 128 > st.limit_min || __any(next.dead)) st.mask(s[B], 64 * u + 64 + 16 * lg, next.dead);
         __builtin_amdgcn_sched_barrier(0);
         st.template values<0, ND, false>([&](int d, int v) { return __builtin_bit_cast(vec8, lds_v[A][(d * 2 + v) * 64 + lane]); }, w);
-        st.peak(s[B], next.kf, top);
+        st.peak(s[B], next.kf, next.vs, top);
         mix<2 * ND * NR, 2 * ND, 1, SMALL ? 2 : 4>();
         __builtin_amdgcn_sched_barrier(0);
         if (nan_found[A] == u + 1) st.note_nan((const unsigned long long*)nan_keys[A], u, lg);
-        if (more) {
-            st.raise(top);
-            st.follow(next.top);
-        }
+        if (more) st.raise(top);
         spread_values(next, u + 1, B);
         spread_keys(A);
         here = next;
@@ -866,7 +835,7 @@ __global__ __launch_bounds__(256, W > 128 ? 1 : 2) void cache_tile_kernel(CacheA
         round(u, std::integral_constant<int, 0>{});
         if (u + 1 < u1) round(u + 1, std::integral_constant<int, 1>{});
     }
-    st.finish();
+    st.put_nan();
     float sum[NR], top[NR];
 #pragma unroll
     for (int r = 0; r < NR; ++r) { sum[r] = rows_sum(st.l[r]); top[r] = st.m[r]; }
