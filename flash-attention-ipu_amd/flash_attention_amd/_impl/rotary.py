@@ -74,9 +74,8 @@ def _call_for(q, k, q_weight, k_weight, table, positions):
     return call
 
 
-def _fwd_impl(q, k, q_weight, k_weight, table, positions, eps, interleaved, call=None):
-    if call is None:
-        call = _call_for(q, k, q_weight, k_weight, table, positions)
+def _fwd_impl(q, k, q_weight, k_weight, table, positions, eps, interleaved):
+    call = _call_for(q, k, q_weight, k_weight, table, positions)
     q_out, k_out = torch.empty_like(q), torch.empty_like(k)          # (the operands' layout: heads inside the rows stay there)
     if call.sizes[0] and call.sizes[1]:
         if call.fwd_strides is None:
@@ -95,9 +94,13 @@ def _fwd_impl(q, k, q_weight, k_weight, table, positions, eps, interleaved, call
     return q_out, k_out
 
 
-def _bwd_impl(q, k, dq_out, dk_out, q_weight, k_weight, table, positions, eps, interleaved, need_q_weight, need_k_weight, call=None):
-    if call is None:
-        call = _call_for(q, k, q_weight, k_weight, table, positions)
+def _bwd_impl(q, k, dq_out, dk_out, q_weight, k_weight, table, positions, eps, interleaved, need_q_weight, need_k_weight):
+    # (not the forward's call: hooks on saved tensors may hand them back with other strides, as torch.autograd.graph.save_on_cpu does)
+    if q.stride(-1) != 1 or k.stride(-1) != 1:
+        q, k = q.contiguous(), k.contiguous()
+    if positions is not None and positions.stride(-1) != 1:
+        positions = positions.contiguous()
+    call = _call_for(q, k, q_weight, k_weight, table, positions)
     if dq_out.stride(-1) != 1 or dk_out.stride(-1) != 1:
         dq_out, dk_out = dq_out.contiguous(), dk_out.contiguous()
     dq, dk = torch.empty_like(q), torch.empty_like(k)
@@ -175,7 +178,7 @@ _op.register_autograd(_op_backward, setup_context=_op_setup)
 def _backward(ctx, dq_out, dk_out):
     q, k, q_weight, k_weight, table, positions = ctx.saved_tensors
     need = ctx.needs_input_grad
-    return (*_bwd_impl(q, k, dq_out, dk_out, q_weight, k_weight, table, positions, ctx.eps, ctx.interleaved, need[2], need[3], ctx.call), None, None, None, None)
+    return (*_bwd_impl(q, k, dq_out, dk_out, q_weight, k_weight, table, positions, ctx.eps, ctx.interleaved, need[2], need[3]), None, None, None, None)
 
 
 _backward_once = once_differentiable(_backward)
@@ -188,8 +191,7 @@ class _QkNormRopeFn(torch.autograd.Function):
     def forward(ctx, q, k, q_weight, k_weight, table, positions, eps, interleaved):
         ctx.save_for_backward(q, k, q_weight, k_weight, table, positions)
         ctx.eps, ctx.interleaved = eps, interleaved
-        ctx.call = call = _call_for(q, k, q_weight, k_weight, table, positions)
-        return _fwd_impl(q, k, q_weight, k_weight, table, positions, eps, interleaved, call)
+        return _fwd_impl(q, k, q_weight, k_weight, table, positions, eps, interleaved)
 
     @staticmethod
     def backward(ctx, dq_out, dk_out):
