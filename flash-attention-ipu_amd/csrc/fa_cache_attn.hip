@@ -202,6 +202,12 @@ __device__ __forceinline__ Place find_place(const CacheAttnParams& p, Items item
 __device__ __forceinline__ int fresh_scalar(int x) { asm volatile("" : "+s"(x)); return x; }
 __device__ __forceinline__ int fresh_lane(int x) { asm volatile("" : "+v"(x)); return x; }
 
+// LDS traffic between the lanes of one wave: what stands before is done before what stands behind (the hardware keeps a wave's order; the compiler has to)
+__device__ __forceinline__ void wave_order() {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
+
 // ---- the arithmetic of one unit for the 16 NR rows of a wave --------------------------------------------------------------------------------
 template <typename T, int W, int NR>
 struct RowState {
@@ -360,12 +366,13 @@ struct RowState {
         }
     }
     // A unit that some rows see only in part holds NaN values: they were taken out of the operands (take_nan) and are noted for the rows that see
-    // them; keys[column]: the unit's keys with NaN in that column
-    __device__ __forceinline__ void note_nan(const unsigned long long* keys, int unit, int lg) {
-        keys += 4 * fresh_lane(lg);
+    // them; keys[4 column ..]: the unit's keys with NaN in that column, sixteen in each of four.  Other lanes wrote them: the caller orders that (wave_order, or a barrier)
+    __device__ __forceinline__ void note_nan(const unsigned short* keys, int unit, int lg) {
+        keys += 16 * fresh_lane(lg);
 #pragma unroll 1
         for (int e = 0; e < 4 * ND; ++e) {
-            const unsigned long long k = keys[16 * (e >> 2) + (e & 3)];
+            unsigned long long k;
+            __builtin_memcpy(&k, __builtin_assume_aligned(keys + 4 * (16 * (e >> 2) + (e & 3)), 8), 8);
 #pragma unroll
             for (int r = 0; r < NR; ++r) {
                 const int see = limit[r] - 64 * unit;
@@ -621,7 +628,11 @@ __global__ __launch_bounds__(256, 2) void cache_rows_kernel(CacheAttnParams p) {
                     if constexpr (decltype(i)::value > 0) load_values(here, decltype(i)::value * VN);
                     part(std::integral_constant<int, decltype(i)::value * VN>{});
                 });
-                if (nan) st.note_nan((const unsigned long long*)nan_keys[wave], u, lg);
+                if (nan) {
+                    wave_order();                          // (every lane's marks stand before any lane reads them, and are read before the next unit's)
+                    st.note_nan(nan_keys[wave], u, lg);
+                    wave_order();
+                }
             }
             if (!more) break;
             if (AHEAD) load_values(next, 0);
@@ -823,7 +834,7 @@ __global__ __launch_bounds__(256, W > 128 ? 1 : 2) void cache_tile_kernel(CacheA
         st.peak(s[B], next.kf, next.vs, top);
         mix<2 * ND * NR, 2 * ND, 1, SMALL ? 2 : 4>();
         __builtin_amdgcn_sched_barrier(0);
-        if (nan_found[A] == u + 1) st.note_nan((const unsigned long long*)nan_keys[A], u, lg);
+        if (nan_found[A] == u + 1) st.note_nan(nan_keys[A], u, lg);
         if (more) st.raise(top);
         spread_values(next, u + 1, B);
         spread_keys(A);
