@@ -12,6 +12,7 @@ import pathlib
 import sysconfig
 
 import torch
+from torch.autograd import forward_ad
 
 _LIB = None
 _LIB_PATH = None
@@ -329,6 +330,12 @@ def stream_of(device: torch.device):
         prev = cur
         torch.cuda.set_device(idx)
     return (_raw_stream(idx) if _raw_stream is not None else torch.cuda.current_stream(idx).cuda_stream), prev
+
+
+def refuse_tangents(name, *tensors):
+    """no forward-mode derivative here: a dual tensor would lose its tangent without a word"""
+    if forward_ad._current_level >= 0 and any(t is not None and t.is_floating_point() and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise ValueError(f"{name} has no forward-mode derivative")
 
 
 def fwd_bhld(q, k, v, out, lse_ptr, num_chunks_q, num_chunks_kv, scale, causal):

@@ -130,17 +130,19 @@ def cache_tables(seq_lens: torch.Tensor, new_lens: torch.Tensor, block_tables: t
     key = (seq_lens.shape, seq_lens.stride(), seq_lens.dtype, new_lens.shape, new_lens.stride(), new_lens.dtype, block_tables.shape, block_tables.stride(), block_tables.dtype,
            free_blocks.shape, free_blocks.stride(), free_blocks.dtype, free_count.shape, free_count.dtype, num_tokens, block_size, inplace)
     sizes = _LAYOUTS.get(key)
-    dev = seq_lens.device
     if sizes is None:
         sizes = _remember(key, _check_tables(seq_lens, new_lens, block_tables, free_blocks, free_count, num_tokens, block_size, inplace))
+    dev = seq_lens.device
     if not (seq_lens.is_cuda and new_lens.device == dev and block_tables.device == dev and free_blocks.device == dev and free_count.device == dev):
         raise ValueError("cache_tables: all tensors must be on one GPU")
     # one allocation: cu_new, granted, positions, slots and, unless in place, lengths and count
     parts = torch.split_with_sizes(seq_lens.new_empty(sizes[0]), sizes[1])
     cu_new, granted, positions, slots = parts[:4]
     seq_out, free_out = (seq_lens, free_count) if inplace else parts[4:]
-    call = _tables_op if torch.compiler.is_compiling() else _tables_call
-    call(seq_lens, new_lens, block_tables, free_blocks, free_count, num_tokens, block_size, seq_out, free_out, cu_new, granted, positions, slots)
+    if torch.compiler.is_compiling():
+        _tables_op(seq_lens, new_lens, block_tables, free_blocks, free_count, num_tokens, block_size, seq_out, free_out, cu_new, granted, positions, slots)
+    else:
+        _tables_call(seq_lens, new_lens, block_tables, free_blocks, free_count, num_tokens, block_size, seq_out, free_out, cu_new, granted, positions, slots)
     return CacheStep(seq_out, free_out, cu_new, granted, positions, slots)
 
 
@@ -230,6 +232,7 @@ def cache_append(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, k_cache:
     """
     if torch.is_grad_enabled() and (k.requires_grad or v.requires_grad):
         raise ValueError("cache_append has no gradient: call it under torch.no_grad()")
+    _native.refuse_tangents("cache_append", k, v, k_cache, v_cache, k_scale, v_scale)
     if torch.compiler.is_compiling():
         return _append_op(k, v, slots, k_cache, v_cache, k_scale, v_scale)
     return _append_call(k, v, slots, k_cache, v_cache, k_scale, v_scale)
@@ -324,6 +327,7 @@ def flash_attention_cached(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torc
         raise ValueError(f"flash_attention_cached: q must be [tokens, heads, head dim] (got {tuple(q.shape)})")
     if torch.is_grad_enabled() and q.requires_grad:
         raise ValueError("flash_attention_cached has no gradient: call it under torch.no_grad()")
+    _native.refuse_tangents("flash_attention_cached", q, k_cache, v_cache, k_scale, v_scale, out)
     if softmax_scale is None:
         softmax_scale = q.shape[2] ** -0.5
     elif not 0.0 < softmax_scale < float("inf"):
