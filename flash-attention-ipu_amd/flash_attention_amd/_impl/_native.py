@@ -332,6 +332,11 @@ def stream_of(device: torch.device):
     return (_raw_stream(idx) if _raw_stream is not None else torch.cuda.current_stream(idx).cuda_stream), prev
 
 
+def through_dispatcher() -> bool:
+    """whether a call has to go through its registered op: it is compiled, traced, or a dispatch mode looks on (eager calls pass the dispatcher by)"""
+    return torch.compiler.is_compiling() or torch._C._len_torch_dispatch_stack() > 0
+
+
 def refuse_tangents(name, *tensors):
     """no forward-mode derivative here: a dual tensor would lose its tangent without a word"""
     if forward_ad._current_level >= 0 and any(t is not None and t.is_floating_point() and forward_ad.unpack_dual(t).tangent is not None for t in tensors):

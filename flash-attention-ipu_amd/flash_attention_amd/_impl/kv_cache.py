@@ -127,11 +127,15 @@ def cache_tables(seq_lens: torch.Tensor, new_lens: torch.Tensor, block_tables: t
     A request is served whole or not at all (granted): its tokens have to end inside num_tokens, its blocks have to fit its table row, and the pool has
     to hold what all such requests up to and including it need.  Nothing is read back: look at `granted` when the host next waits for the device.
     """
-    key = (seq_lens.shape, seq_lens.stride(), seq_lens.dtype, new_lens.shape, new_lens.stride(), new_lens.dtype, block_tables.shape, block_tables.stride(), block_tables.dtype,
-           free_blocks.shape, free_blocks.stride(), free_blocks.dtype, free_count.shape, free_count.dtype, num_tokens, block_size, inplace)
-    sizes = _LAYOUTS.get(key)
-    if sizes is None:
-        sizes = _remember(key, _check_tables(seq_lens, new_lens, block_tables, free_blocks, free_count, num_tokens, block_size, inplace))
+    dispatch = _native.through_dispatcher()
+    if dispatch:
+        sizes = _check_tables(seq_lens, new_lens, block_tables, free_blocks, free_count, num_tokens, block_size, inplace)
+    else:
+        key = (seq_lens.shape, seq_lens.stride(), seq_lens.dtype, new_lens.shape, new_lens.stride(), new_lens.dtype, block_tables.shape, block_tables.stride(), block_tables.dtype,
+               free_blocks.shape, free_blocks.stride(), free_blocks.dtype, free_count.shape, free_count.dtype, num_tokens, block_size, inplace)
+        sizes = _LAYOUTS.get(key)
+        if sizes is None:
+            sizes = _remember(key, _check_tables(seq_lens, new_lens, block_tables, free_blocks, free_count, num_tokens, block_size, inplace))
     dev = seq_lens.device
     if not (seq_lens.is_cuda and new_lens.device == dev and block_tables.device == dev and free_blocks.device == dev and free_count.device == dev):
         raise ValueError("cache_tables: all tensors must be on one GPU")
@@ -139,7 +143,7 @@ def cache_tables(seq_lens: torch.Tensor, new_lens: torch.Tensor, block_tables: t
     parts = torch.split_with_sizes(seq_lens.new_empty(sizes[0]), sizes[1])
     cu_new, granted, positions, slots = parts[:4]
     seq_out, free_out = (seq_lens, free_count) if inplace else parts[4:]
-    if torch.compiler.is_compiling():
+    if dispatch:
         _tables_op(seq_lens, new_lens, block_tables, free_blocks, free_count, num_tokens, block_size, seq_out, free_out, cu_new, granted, positions, slots)
     else:
         _tables_call(seq_lens, new_lens, block_tables, free_blocks, free_count, num_tokens, block_size, seq_out, free_out, cu_new, granted, positions, slots)
@@ -233,7 +237,7 @@ def cache_append(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, k_cache:
     if torch.is_grad_enabled() and (k.requires_grad or v.requires_grad):
         raise ValueError("cache_append has no gradient: call it under torch.no_grad()")
     _native.refuse_tangents("cache_append", k, v, k_cache, v_cache, k_scale, v_scale)
-    if torch.compiler.is_compiling():
+    if _native.through_dispatcher():
         return _append_op(k, v, slots, k_cache, v_cache, k_scale, v_scale)
     return _append_call(k, v, slots, k_cache, v_cache, k_scale, v_scale)
 
@@ -334,7 +338,7 @@ def flash_attention_cached(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torc
         raise ValueError(f"flash_attention_cached: softmax_scale must be finite and > 0 (got {softmax_scale})")
     if max_q_len is None:
         max_q_len = max(1, q.shape[0] - seq_lens.shape[0] + 1) if seq_lens.ndim == 1 else 1
-    if torch.compiler.is_compiling():
+    if _native.through_dispatcher():
         if out is None:
             out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
         _attn_op(q, k_cache, v_cache, k_scale, v_scale, block_tables, seq_lens, cu_q, softmax_scale, max_q_len, out)

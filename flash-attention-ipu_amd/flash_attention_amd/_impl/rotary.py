@@ -251,7 +251,7 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: Optional[torch.Tens
     if positions is not None and positions.ndim and positions.stride(-1) != 1:
         positions = positions.contiguous()
     _native.refuse_tangents("qk_norm_rope", q, k, q_weight, k_weight, table)
-    if torch.compiler.is_compiling():
+    if _native.through_dispatcher():
         _check(q, k, q_weight, k_weight, table, positions)
         return _op(q, k, q_weight, k_weight, table, positions, float(eps), bool(interleaved))
     if torch.is_grad_enabled():

@@ -1,11 +1,57 @@
-"""CPU tests: the cache and rotation operators under forward-mode levels (no kernel runs)."""
+"""CPU tests: the cache and rotation operators under dispatch modes, tracers and forward-mode levels (fake GPU tensors; no kernel runs)."""
 
 import pytest
 import torch
+from torch._subclasses.fake_tensor import FakeTensorMode
 from torch.autograd import forward_ad
+from torch.fx.experimental.proxy_tensor import make_fx
+from torch.utils._python_dispatch import TorchDispatchMode
 
 import flash_attention_amd.kv_cache as kv
 import flash_attention_amd.rotary as rot
+
+
+class Log(TorchDispatchMode):
+    def __init__(self):
+        super().__init__()
+        self.names = []
+
+    def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+        self.names.append(func._schema.name)
+        return func(*args, **(kwargs or {}))
+
+
+def half(*shape, **kw):
+    return torch.empty(*shape, device="cuda", dtype=torch.float16, **kw)
+
+
+def step_of_a_layer(cache, new, q, k, v, table):
+    step = cache.step(new, q.shape[0])
+    q, k = rot.qk_norm_rope(q, k, None, None, table, step.positions)
+    return cache.attend(0, q, k, v, step)
+
+
+def inputs():
+    cache = kv.KVCache(1, 8, 2, 64, requests=2, max_tokens=64, block_size=16)
+    return cache, torch.empty(2, device="cuda", dtype=torch.int32), half(5, 4, 64), half(5, 2, 64), half(5, 2, 64), torch.empty(64, 64, device="cuda")
+
+
+OPS = ["flash_attention_amd::cache_tables", "flash_attention_amd::qk_norm_rope", "flash_attention_amd::cache_append", "flash_attention_amd::cached"]
+
+
+def test_a_dispatch_mode_sees_the_operators():
+    with FakeTensorMode():
+        args = inputs()
+        with Log() as log:
+            out = step_of_a_layer(*args)
+    assert out.shape == (5, 4, 64) and [n for n in log.names if n.startswith("flash_attention_amd")] == OPS
+
+
+def test_a_tracer_sees_the_operators():
+    with FakeTensorMode():
+        cache, *args = inputs()
+        graph = make_fx(lambda *a: step_of_a_layer(cache, *a))(*args)
+    assert [n.target.name().rsplit(".", 1)[0] for n in graph.graph.nodes if "flash_attention_amd" in str(n.target)] == OPS
 
 
 def test_tangents_are_refused():
