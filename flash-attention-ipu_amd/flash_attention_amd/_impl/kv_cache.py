@@ -7,6 +7,7 @@ import ctypes
 from typing import NamedTuple, Optional
 
 import torch
+from torch.autograd.graph import increment_version
 from torch.library import custom_op
 
 from . import _native
@@ -147,6 +148,7 @@ def cache_tables(seq_lens: torch.Tensor, new_lens: torch.Tensor, block_tables: t
         _tables_op(seq_lens, new_lens, block_tables, free_blocks, free_count, num_tokens, block_size, seq_out, free_out, cu_new, granted, positions, slots)
     else:
         _tables_call(seq_lens, new_lens, block_tables, free_blocks, free_count, num_tokens, block_size, seq_out, free_out, cu_new, granted, positions, slots)
+        increment_version((block_tables, free_blocks, seq_lens, free_count) if inplace else (block_tables, free_blocks))
     return CacheStep(seq_out, free_out, cu_new, granted, positions, slots)
 
 
@@ -239,7 +241,8 @@ def cache_append(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, k_cache:
     _native.refuse_tangents("cache_append", k, v, k_cache, v_cache, k_scale, v_scale)
     if _native.through_dispatcher():
         return _append_op(k, v, slots, k_cache, v_cache, k_scale, v_scale)
-    return _append_call(k, v, slots, k_cache, v_cache, k_scale, v_scale)
+    _append_call(k, v, slots, k_cache, v_cache, k_scale, v_scale)
+    increment_version((k_cache, v_cache, k_scale, v_scale))
 
 
 def _attn_call(q, k_cache, v_cache, k_scale, v_scale, block_tables, seq_lens, cu_q, softmax_scale, max_q_len, out):
@@ -343,7 +346,11 @@ def flash_attention_cached(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torc
             out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
         _attn_op(q, k_cache, v_cache, k_scale, v_scale, block_tables, seq_lens, cu_q, softmax_scale, max_q_len, out)
         return out
-    return _attn_call(q, k_cache, v_cache, k_scale, v_scale, block_tables, seq_lens, cu_q, softmax_scale, max_q_len, out)
+    if out is None:
+        return _attn_call(q, k_cache, v_cache, k_scale, v_scale, block_tables, seq_lens, cu_q, softmax_scale, max_q_len, None)
+    _attn_call(q, k_cache, v_cache, k_scale, v_scale, block_tables, seq_lens, cu_q, softmax_scale, max_q_len, out)
+    increment_version(out)
+    return out
 
 
 class KVCache:

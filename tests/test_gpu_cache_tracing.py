@@ -9,6 +9,24 @@ pytestmark = pytest.mark.gpu
 DEV = "cuda"
 
 
+@pytest.fixture(scope="module")
+def kv():
+    import flash_attention_amd.kv_cache as kv
+
+    return kv
+
+
+@pytest.fixture(scope="module")
+def rot():
+    import flash_attention_amd.rotary as rot
+
+    return rot
+
+
+def ints(x):
+    return torch.tensor(x, dtype=torch.int32, device=DEV)
+
+
 def test_a_traced_step_runs(kv, rot):
     """the graph that a tracer records of a step does what the step does"""
     g = torch.Generator().manual_seed(0)
@@ -50,3 +68,40 @@ def test_the_backward_is_dispatched(rot):
         got = run()
     assert [n for n in log.names if n.startswith("flash")] == ["flash_attention_amd::qk_norm_rope", "flash_attention_amd::qk_norm_rope_bwd"]
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_changed_tensors_say_so(kv):
+    """version counters: a tensor that a call writes and a graph has saved is noticed"""
+    cache = kv.KVCache(1, 8, 2, 64, requests=2, max_tokens=64, block_size=16)
+    layer = cache._layer[0]
+    q, k = torch.zeros(3, 4, 64, dtype=torch.float16, device=DEV), torch.zeros(3, 2, 64, dtype=torch.float16, device=DEV)
+    state = (cache.block_tables, cache.free_blocks, cache.seq_lens, cache.free_count)
+    before = [t._version for t in state]
+    step = cache.step(ints([2, 1]), 3)
+    assert all(t._version > n for t, n in zip(state, before))
+    before = [t._version for t in state]
+    kv.cache_tables(cache.seq_lens, ints([0, 0]), cache.block_tables, cache.free_blocks, cache.free_count, 3, 16)
+    assert [t._version > n for t, n in zip(state, before)] == [True, True, False, False]
+    before = [t._version for t in layer]
+    cache.append(0, k, k, step)
+    assert all(t._version > n for t, n in zip(layer, before)) and cache.k_cache._version == layer[0]._version
+    out = torch.empty_like(q)
+    before, read = out._version, [t._version for t in (q, *layer, cache.block_tables)]
+    kv.flash_attention_cached(q, *layer, cache.block_tables, step.seq_lens, step.cu_new, out=out)
+    assert out._version > before and [t._version for t in (q, *layer, cache.block_tables)] == read
+    rows, table = torch.arange(2, device=DEV), torch.ones(65, 4, device=DEV, requires_grad=True)
+    picked = table[cache.seq_lens.clamp_(max=64)] * table[rows]
+    cache.step(ints([1, 1]), 2)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        picked.sum().backward()
+
+
+def test_calls_in_inference_mode(kv, rot):
+    """tensors without version counters"""
+    with torch.inference_mode():
+        cache = kv.KVCache(1, 8, 2, 64, requests=2, max_tokens=64, block_size=16)
+        q, k, v = (torch.randn(3, h, 64, device=DEV).half() for h in (4, 2, 2))
+        step = cache.step(ints([2, 1]), 3)
+        q, k = rot.qk_norm_rope(q, k, None, None, rot.rotary_table(64, 64, device=DEV), step.positions)
+        out = cache.attend(0, q, k, v, step, out=torch.empty_like(q))
+    assert bool(torch.isfinite(out).all()) and cache.seq_lens.tolist() == [2, 1]
