@@ -236,7 +236,7 @@ def cache_append(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, k_cache:
     largest value; later runs raise it where they need to, and the block's codes are brought along.  inf and NaN are stored as NaN.  One call may bring
     one run to a block: two runs in one block, or a slot twice, leave that block's contents unspecified.
     """
-    if torch.is_grad_enabled() and (k.requires_grad or v.requires_grad):
+    if torch.is_grad_enabled() and (k.requires_grad or v.requires_grad or k_cache.requires_grad or v_cache.requires_grad or k_scale.requires_grad or v_scale.requires_grad):
         raise ValueError("cache_append has no gradient: call it under torch.no_grad()")
     _native.refuse_tangents("cache_append", k, v, k_cache, v_cache, k_scale, v_scale)
     if _native.through_dispatcher():
@@ -332,7 +332,8 @@ def flash_attention_cached(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torc
     """
     if q.ndim != 3:
         raise ValueError(f"flash_attention_cached: q must be [tokens, heads, head dim] (got {tuple(q.shape)})")
-    if torch.is_grad_enabled() and q.requires_grad:
+    if torch.is_grad_enabled() and (q.requires_grad or k_cache.requires_grad or v_cache.requires_grad or k_scale.requires_grad or v_scale.requires_grad
+                                    or (out is not None and out.requires_grad)):
         raise ValueError("flash_attention_cached has no gradient: call it under torch.no_grad()")
     _native.refuse_tangents("flash_attention_cached", q, k_cache, v_cache, k_scale, v_scale, out)
     if softmax_scale is None:

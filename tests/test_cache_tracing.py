@@ -75,3 +75,15 @@ def test_tangents_are_refused():
                 kv.flash_attention_cached(*args, torch.zeros(1, 1, dtype=torch.int32), ints[:1], ints[:2])
         with pytest.raises((ValueError, TypeError), match="GPU"):          # (no tangent: the other checks)
             rot.qk_norm_rope(x, x, None, None, table)
+
+
+def test_gradients_that_nothing_forms_are_refused():
+    x, ints, ones = torch.zeros(4, 2, 64, dtype=torch.float16), torch.zeros(4, dtype=torch.int32), torch.ones(4, 2)
+    codes = [torch.zeros(4, 2, *s, dtype=torch.uint8).view(torch.float8_e4m3fn) for s in ((16, 64), (64, 16))]
+    wants = ones.clone().requires_grad_()
+    with pytest.raises(ValueError, match="no gradient"):
+        kv.cache_append(x, x, ints, *codes, wants, ones)
+    for kw in (dict(k_scale=wants), dict(v_scale=wants), dict(out=x.clone().requires_grad_())):
+        with pytest.raises(ValueError, match="no gradient"):
+            kv.flash_attention_cached(**{**dict(q=x, k_cache=codes[0], v_cache=codes[1], k_scale=ones, v_scale=ones, block_tables=torch.zeros(1, 1, dtype=torch.int32),
+                                                seq_lens=ints[:1], cu_q=ints[:2]), **kw})
