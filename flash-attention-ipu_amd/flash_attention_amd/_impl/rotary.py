@@ -250,13 +250,13 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: Optional[torch.Tens
         q, k = q.contiguous(), k.contiguous()
     if positions is not None and positions.ndim and positions.stride(-1) != 1:
         positions = positions.contiguous()
+    grad = torch.is_grad_enabled()
+    if grad and table.requires_grad:
+        raise ValueError("qk_norm_rope has no gradient for the table")
     _native.refuse_tangents("qk_norm_rope", q, k, q_weight, k_weight, table)
     if _native.through_dispatcher():
         _check(q, k, q_weight, k_weight, table, positions)
         return _op(q, k, q_weight, k_weight, table, positions, float(eps), bool(interleaved))
-    if torch.is_grad_enabled():
-        if table.requires_grad:
-            raise ValueError("qk_norm_rope has no gradient for the table")
-        if q.requires_grad or k.requires_grad or (q_weight is not None and q_weight.requires_grad) or (k_weight is not None and k_weight.requires_grad):
-            return _QkNormRopeFn.apply(q, k, q_weight, k_weight, table, positions, eps, interleaved)
+    if grad and (q.requires_grad or k.requires_grad or (q_weight is not None and q_weight.requires_grad) or (k_weight is not None and k_weight.requires_grad)):
+        return _QkNormRopeFn.apply(q, k, q_weight, k_weight, table, positions, eps, interleaved)
     return _fwd_impl(q, k, q_weight, k_weight, table, positions, eps, interleaved)

@@ -87,3 +87,20 @@ def test_gradients_that_nothing_forms_are_refused():
         with pytest.raises(ValueError, match="no gradient"):
             kv.flash_attention_cached(**{**dict(q=x, k_cache=codes[0], v_cache=codes[1], k_scale=ones, v_scale=ones, block_tables=torch.zeros(1, 1, dtype=torch.int32),
                                                 seq_lens=ints[:1], cu_q=ints[:2]), **kw})
+
+
+def test_a_table_that_wants_a_gradient_is_refused():
+    """eager, under a dispatch mode and compiled alike"""
+    table = torch.zeros(8, 64, requires_grad=True)
+    x = torch.zeros(4, 2, 64)
+    with pytest.raises(ValueError, match="no gradient for the table"):
+        rot.qk_norm_rope(x, x, None, None, table)
+    with FakeTensorMode():
+        q, table = half(4, 2, 64), torch.empty(8, 64, device="cuda", requires_grad=True)
+        with pytest.raises(ValueError, match="no gradient for the table"):
+            rot.qk_norm_rope(q, q, None, None, table)
+        with torch.no_grad():
+            rot.qk_norm_rope(q, q, None, None, table)
+    compiled = torch.compile(lambda t: rot.qk_norm_rope(x, x, None, None, t), backend="eager")
+    with pytest.raises(Exception, match="no gradient for the table"):
+        compiled(torch.zeros(8, 64, requires_grad=True))
