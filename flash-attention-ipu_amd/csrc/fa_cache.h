@@ -86,6 +86,7 @@ struct CacheAttnParams {
     const int32_t* tables;  // [B][width]
     const int32_t* seq_lens;// [B]
     const int32_t* cu_q;    // [B + 1]
+    const int32_t* granted; // [B] or null; 0 = the request's rows see nothing
     float* ws_o;            // partial sums, see fa_cache_attn.hip
     float* ws_ml;
     long long* ws_prefix;   // [B + 1]

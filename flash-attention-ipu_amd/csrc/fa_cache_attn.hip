@@ -129,6 +129,7 @@ __device__ __forceinline__ Request request_of(const CacheAttnParams& p, int b) {
     r.n = e - a;
     r.len = max(constant(p.seq_lens + b), 0);
     r.len = r.len < room ? r.len : (int)room;
+    if (p.granted && constant(p.granted + b) <= 0) r.len = 0;      // (rows whose own tokens are not in the cache)
     r.units = max(1, (int)(((long long)r.len + 63) >> 6));
     return r;
 }

@@ -316,6 +316,14 @@ int fa_cache_attn(const void* q, void* out, const void* k_cache, const void* v_c
                   const int32_t* seq_lens, const int32_t* cu_q, void* workspace, int64_t workspace_bytes, int64_t num_requests, int64_t num_tokens, int64_t heads,
                   int64_t heads_kv, int64_t D, int64_t W, int64_t num_blocks, int64_t block_size, int64_t max_blocks, int64_t table_stride, int64_t max_q_len,
                   const int64_t token_strides[4], const int64_t block_strides[4], int32_t dtype, float softmax_scale, void* stream) {
+    return fa_cache_attn_granted(q, out, k_cache, v_cache, k_scale, v_scale, block_tables, seq_lens, cu_q, nullptr, workspace, workspace_bytes, num_requests, num_tokens, heads,
+                                 heads_kv, D, W, num_blocks, block_size, max_blocks, table_stride, max_q_len, token_strides, block_strides, dtype, softmax_scale, stream);
+}
+
+int fa_cache_attn_granted(const void* q, void* out, const void* k_cache, const void* v_cache, const float* k_scale, const float* v_scale, const int32_t* block_tables,
+                          const int32_t* seq_lens, const int32_t* cu_q, const int32_t* granted, void* workspace, int64_t workspace_bytes, int64_t num_requests, int64_t num_tokens, int64_t heads,
+                          int64_t heads_kv, int64_t D, int64_t W, int64_t num_blocks, int64_t block_size, int64_t max_blocks, int64_t table_stride, int64_t max_q_len,
+                          const int64_t token_strides[4], const int64_t block_strides[4], int32_t dtype, float softmax_scale, void* stream) {
     if (!q || !out || !k_cache || !v_cache || !k_scale || !v_scale || !block_tables || !seq_lens || !cu_q || !token_strides || !block_strides)
         return fail(FA_ERR_NULL_POINTER, "fa_cache_attn: null pointer");
     if (dtype != FA_DTYPE_F16 && dtype != FA_DTYPE_BF16) return fail(FA_ERR_BAD_DTYPE, "queries must be FA_DTYPE_F16 or FA_DTYPE_BF16 (got %d)", dtype);
@@ -334,7 +342,7 @@ int fa_cache_attn(const void* q, void* out, const void* k_cache, const void* v_c
         return fail(FA_ERR_WORKSPACE, "fa_cache_attn: workspace must be 16-byte aligned and hold %lld bytes", (long long)plan.bytes);
     fa::CacheAttnParams p{};
     p.q = q; p.o = out; p.k = (const uint8_t*)k_cache; p.v = (const uint8_t*)v_cache; p.ks = k_scale; p.vs = v_scale;
-    p.tables = block_tables; p.seq_lens = seq_lens; p.cu_q = cu_q;
+    p.tables = block_tables; p.seq_lens = seq_lens; p.cu_q = cu_q; p.granted = granted;
     if (plan.bytes) {
         p.ws_o = (float*)((char*)workspace + plan.ws_o);
         p.ws_ml = (float*)((char*)workspace + plan.ws_ml);

@@ -124,6 +124,8 @@ def _declare(lib):
     lib.fa_cache_attn_workspace.argtypes = [i64] * 8
     lib.fa_cache_attn.restype = ctypes.c_int
     lib.fa_cache_attn.argtypes = [vp] * 10 + [i64] * 12 + [vp, vp, i32, f32, vp]
+    lib.fa_cache_attn_granted.restype = ctypes.c_int
+    lib.fa_cache_attn_granted.argtypes = [vp] * 11 + [i64] * 12 + [vp, vp, i32, f32, vp]
 
 
 def _raise(rc):

@@ -245,11 +245,12 @@ def cache_append(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, k_cache:
     increment_version((k_cache, v_cache, k_scale, v_scale))
 
 
-def _attn_call(q, k_cache, v_cache, k_scale, v_scale, block_tables, seq_lens, cu_q, softmax_scale, max_q_len, out):
+def _attn_call(q, k_cache, v_cache, k_scale, v_scale, block_tables, seq_lens, cu_q, softmax_scale, max_q_len, out, granted):
     name = "flash_attention_cached"
     key = (q.shape, q.stride(), q.dtype, None if out is None else (out.shape, out.stride(), out.dtype), max_q_len, k_cache.shape, k_cache.stride(), v_cache.shape, v_cache.stride(), k_cache.dtype,
            v_cache.dtype, k_scale.shape, k_scale.stride(), v_scale.shape, v_scale.stride(), k_scale.dtype, v_scale.dtype, block_tables.shape, block_tables.stride(),
-           block_tables.dtype, seq_lens.shape, seq_lens.stride(), seq_lens.dtype, cu_q.shape, cu_q.stride(), cu_q.dtype)
+           block_tables.dtype, seq_lens.shape, seq_lens.stride(), seq_lens.dtype, cu_q.shape, cu_q.stride(), cu_q.dtype,
+           None if granted is None else (granted.shape, granted.stride(), granted.dtype))
     lib = _native._LIB or _native.load_native_library()
     known = _LAYOUTS.get(key)
     if known is None:
@@ -269,6 +270,8 @@ def _attn_call(q, k_cache, v_cache, k_scale, v_scale, block_tables, seq_lens, cu
             raise ValueError(f"{name}: seq_lens must be [requests] (got {tuple(seq_lens.shape)})")
         B = seq_lens.shape[0]
         _ints(name, "cu_q", cu_q, (B + 1,))
+        if granted is not None:
+            _ints(name, "granted", granted, (B,))
         width, table_stride = _table(name, block_tables, B)
         if max_q_len < 1:
             raise ValueError(f"{name}: max_q_len must be >= 1 (got {max_q_len})")
@@ -283,7 +286,7 @@ def _attn_call(q, k_cache, v_cache, k_scale, v_scale, block_tables, seq_lens, cu
     if out is None:
         out = torch.empty_like(q) if q.is_contiguous() else torch.empty(q.shape, dtype=q.dtype, device=dev)     # (the first takes half the time)
     if not (q.is_cuda and dev == out.device == k_cache.device == v_cache.device == k_scale.device == v_scale.device == block_tables.device == seq_lens.device
-            == cu_q.device):
+            == cu_q.device and (granted is None or granted.device == dev)):
         raise ValueError(f"{name}: all tensors must be on one GPU")
     if out.data_ptr() % 16:
         raise ValueError(f"{name}: out must be 16-byte aligned")
@@ -296,8 +299,9 @@ def _attn_call(q, k_cache, v_cache, k_scale, v_scale, block_tables, seq_lens, cu
     ws = seq_lens.new_empty((nbytes + 3) // 4) if nbytes else None
     stream, prev = _native.stream_of(dev)
     try:
-        rc = lib.fa_cache_attn(q.data_ptr(), out.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), block_tables.data_ptr(),
-                               seq_lens.data_ptr(), cu_q.data_ptr(), None if ws is None else ws.data_ptr(), nbytes, *sizes, tokens, strides, dtype, softmax_scale, stream)
+        rc = lib.fa_cache_attn_granted(q.data_ptr(), out.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), block_tables.data_ptr(),
+                                       seq_lens.data_ptr(), cu_q.data_ptr(), None if granted is None else granted.data_ptr(), None if ws is None else ws.data_ptr(), nbytes,
+                                       *sizes, tokens, strides, dtype, softmax_scale, stream)
     finally:
         if prev >= 0:
             torch.cuda.set_device(prev)
@@ -308,13 +312,13 @@ def _attn_call(q, k_cache, v_cache, k_scale, v_scale, block_tables, seq_lens, cu
 
 @custom_op("flash_attention_amd::cached", mutates_args=("out",))
 def _attn_op(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor, block_tables: torch.Tensor,
-             seq_lens: torch.Tensor, cu_q: torch.Tensor, softmax_scale: float, max_q_len: int, out: torch.Tensor) -> None:
-    _attn_call(q, k_cache, v_cache, k_scale, v_scale, block_tables, seq_lens, cu_q, softmax_scale, max_q_len, out)
+             seq_lens: torch.Tensor, cu_q: torch.Tensor, softmax_scale: float, max_q_len: int, out: torch.Tensor, granted: Optional[torch.Tensor] = None) -> None:
+    _attn_call(q, k_cache, v_cache, k_scale, v_scale, block_tables, seq_lens, cu_q, softmax_scale, max_q_len, out, granted)
 
 
 def flash_attention_cached(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor, block_tables: torch.Tensor,
                            seq_lens: torch.Tensor, cu_q: torch.Tensor, softmax_scale: Optional[float] = None, max_q_len: Optional[int] = None,
-                           out: Optional[torch.Tensor] = None) -> torch.Tensor:
+                           out: Optional[torch.Tensor] = None, granted: Optional[torch.Tensor] = None) -> torch.Tensor:
     """
     Causal attention of a step's queries over the cached keys and values of their requests; for inference (no gradient).
 
@@ -328,6 +332,8 @@ def flash_attention_cached(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torc
                  is a step of single tokens.  Give prompts and single tokens calls of their own where both are many: one long cache is split over
                  the chip by the kernel for single tokens only.
     out          [T, heads, D], default a new tensor.  Rows behind cu_q[B] are not written: a new tensor holds anything there.
+    granted      int32 [B] (CacheStep.granted): the rows of a request that was refused, whose tokens are not in the cache, give zeros.  Default: every request counts
+                 as served, and the rows of a refused one as the last tokens of what it holds.
     returns      out.  A query that sees no key (an empty request) gives zeros.
     """
     if q.ndim != 3:
@@ -345,11 +351,11 @@ def flash_attention_cached(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torc
     if _native.through_dispatcher():
         if out is None:
             out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        _attn_op(q, k_cache, v_cache, k_scale, v_scale, block_tables, seq_lens, cu_q, softmax_scale, max_q_len, out)
+        _attn_op(q, k_cache, v_cache, k_scale, v_scale, block_tables, seq_lens, cu_q, softmax_scale, max_q_len, out, granted)
         return out
     if out is None:
-        return _attn_call(q, k_cache, v_cache, k_scale, v_scale, block_tables, seq_lens, cu_q, softmax_scale, max_q_len, None)
-    _attn_call(q, k_cache, v_cache, k_scale, v_scale, block_tables, seq_lens, cu_q, softmax_scale, max_q_len, out)
+        return _attn_call(q, k_cache, v_cache, k_scale, v_scale, block_tables, seq_lens, cu_q, softmax_scale, max_q_len, None, granted)
+    _attn_call(q, k_cache, v_cache, k_scale, v_scale, block_tables, seq_lens, cu_q, softmax_scale, max_q_len, out, granted)
     increment_version(out)
     return out
 
@@ -391,6 +397,6 @@ class KVCache:
 
     def attend(self, layer: int, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, step: CacheStep, softmax_scale: Optional[float] = None,
                max_q_len: Optional[int] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
-        """the step's keys and values into the layer's cache, then its queries' attention"""
+        """the step's keys and values into the layer's cache, then its queries' attention (zeros for a request that was refused)"""
         self.append(layer, k, v, step)
-        return flash_attention_cached(q, *self._layer[layer], self.block_tables, step.seq_lens, step.cu_new, softmax_scale, max_q_len, out)
+        return flash_attention_cached(q, *self._layer[layer], self.block_tables, step.seq_lens, step.cu_new, softmax_scale, max_q_len, out, step.granted)

@@ -354,6 +354,13 @@ int fa_cache_attn(const void* q, void* out, const void* k_cache, const void* v_c
                   const int32_t* seq_lens, const int32_t* cu_q, void* workspace, int64_t workspace_bytes, int64_t num_requests, int64_t num_tokens, int64_t heads,
                   int64_t heads_kv, int64_t D, int64_t W, int64_t num_blocks, int64_t block_size, int64_t max_blocks, int64_t table_stride, int64_t max_q_len,
                   const int64_t token_strides[4], const int64_t block_strides[4], int32_t dtype, float softmax_scale, void* stream);
+/* The same with fa_cache_tables' `granted` [B] (or NULL): a request that was refused keeps its rows in cu_q but has none of their tokens in the cache.  Where
+ * granted[b] is 0, its rows see no key: zeros, and the cache is not read for them.  (Without it they count as the last tokens of what the request holds.) */
+int fa_cache_attn_granted(const void* q, void* out, const void* k_cache, const void* v_cache, const float* k_scale, const float* v_scale, const int32_t* block_tables,
+                          const int32_t* seq_lens, const int32_t* cu_q, const int32_t* granted, void* workspace, int64_t workspace_bytes, int64_t num_requests,
+                          int64_t num_tokens, int64_t heads, int64_t heads_kv, int64_t D, int64_t W, int64_t num_blocks, int64_t block_size, int64_t max_blocks,
+                          int64_t table_stride, int64_t max_q_len, const int64_t token_strides[4], const int64_t block_strides[4], int32_t dtype, float softmax_scale,
+                          void* stream);
 
 #ifdef __cplusplus
 }

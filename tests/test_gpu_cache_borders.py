@@ -4,7 +4,8 @@ import numpy as np
 import pytest
 import torch
 
-from test_gpu_kv_cache import check_attention
+from kv_cache_reference import attention_reference
+from test_gpu_kv_cache import DEV, check_attention, code_values, ints, tolerance
 
 pytestmark = pytest.mark.gpu
 
@@ -36,3 +37,41 @@ def test_nan_marks_of_one_request_after_the_other(kv, dtype, P, D, max_q_len):
 
     out = check_attention(kv, held, [2] * 400, 2, 2, D, P, dtype, seed=31, max_q_len=max_q_len, poke=poke)
     assert not bool(torch.isnan(out[0::2]).any()) and int(torch.isnan(out[1::2]).sum()) == 2 * sum(b % 3 != 2 for b in range(400))
+
+
+@BOTH
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("hint", [1, 1000])
+@pytest.mark.parametrize("why", ["pool", "table", "tokens", "long"])
+def test_refused_requests_between_served_ones(kv, dtype, D, hint, why):
+    """rows whose tokens found no place: zeros; the others' attention, the cache and a later step are as if they had not been there"""
+    Hkv, H, P, g = 2, 4, 16, torch.Generator().manual_seed(41)
+    blocks, most, held, new, served, room = {
+        "pool": (10, 128, [40, 30, 20, 0], [1, 60, 5, 2], [1, 0, 5, 0], 70),
+        "table": (60, 64, [40, 30, 20, 0], [1, 60, 5, 2], [1, 0, 5, 2], 68),
+        "tokens": (60, 128, [40, 30, 20, 0], [1, 60, 5, 20], [1, 60, 5, 0], 76),
+        "long": (700, 5040, [4900, 5000, 100], [2, 90, 1], [2, 0, 1], 95)}[why]
+    cache = kv.KVCache(1, blocks, Hkv, D, requests=len(held), max_tokens=most, block_size=P)
+    draw = lambda n: [torch.randn(n, h, D, generator=g).to(dtype) for h in (H, Hkv, Hkv)]  # noqa: E731
+    q, k, v = draw(sum(held))
+    cache.append(0, k.to(DEV), v.to(DEV), cache.step(ints(held), sum(held)))
+    q, k, v = draw(room)
+    step = cache.step(ints(new), room)
+    out = torch.full((room, H, D), 7.0, dtype=dtype, device=DEV)
+    cache.attend(0, q.to(DEV), k.to(DEV), v.to(DEV), step, max_q_len=hint, out=out)
+    assert step.granted.tolist() == served and cache.seq_lens.tolist() == [h + s for h, s in zip(held, served)]
+    cu = np.minimum(np.concatenate([[0], np.cumsum(new)]), room).tolist()
+    lens = [h + s if s else 0 for h, s in zip(held, served)]
+    k_cache, v_cache, ks, vs = cache._layer[0]
+    ref, mag = attention_reference(q.double(), code_values(k_cache), code_values(v_cache).transpose(2, 3), ks.cpu().double(), vs.cpu().double(), cache.block_tables.tolist(), lens, cu,
+                                   D ** -0.5)
+    assert bool((out[cu[-1]:] == 7.0).all())
+    out, ref, mag = out[: cu[-1]].cpu().double(), ref[: cu[-1]], mag[: cu[-1]]
+    assert bool(((out - ref).abs() <= tolerance(dtype, ref, mag, 448 * float(vs.max()), max(lens))).all())
+    for b, s in enumerate(served):
+        rows = out[cu[b]:cu[b + 1]]
+        assert bool((rows == 0).all()) if s == 0 else float(rows.abs().min()) >= 0 and float(rows.abs().max()) > 0
+    with pytest.raises((ValueError, TypeError)):
+        kv.flash_attention_cached(q.to(DEV), k_cache, v_cache, ks, vs, cache.block_tables, step.seq_lens, step.cu_new, granted=step.granted.long())
+    with pytest.raises((ValueError, TypeError)):
+        kv.flash_attention_cached(q.to(DEV), k_cache, v_cache, ks, vs, cache.block_tables, step.seq_lens, step.cu_new, granted=step.granted[1:])
