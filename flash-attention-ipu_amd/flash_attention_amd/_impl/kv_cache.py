@@ -328,9 +328,10 @@ def flash_attention_cached(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torc
     cu_q         int32 [B + 1]: request b's queries are the rows cu_q[b] .. cu_q[b + 1] - 1 of q, the last of its seq_lens[b] tokens
                  (CacheStep.cu_new).  A query sees the keys up to its own position.
     softmax_scale  default D ** -0.5
-    max_q_len    the most queries of one request, as far as the host knows; chooses the kernel, never the result.  Default: what T and B allow, so that T == B
-                 is a step of single tokens.  Give prompts and single tokens calls of their own where both are many: one long cache is split over
-                 the chip by the kernel for single tokens only.
+    max_q_len    the most queries of one request, as far as the host knows; chooses the kernel, never the result.  Default: max(1, T - B + 1), a guess that holds where
+                 every request has a token: T == B is a step of single tokens.  Where rows of the batch are idle (no tokens in this step) a prompt can be longer: say
+                 so, or it runs on the kernel for few rows, which reads the request's cache once for every 16 or 32 of its rows.  Give prompts and single tokens calls of
+                 their own where both are many: one long cache is split over the chip by the kernel for single tokens only.
     out          [T, heads, D], default a new tensor.  Rows behind cu_q[B] are not written: a new tensor holds anything there.
     granted      int32 [B] (CacheStep.granted): the rows of a request that was refused, whose tokens are not in the cache, give zeros.  Default: every request counts
                  as served, and the rows of a refused one as the last tokens of what it holds.
@@ -397,6 +398,7 @@ class KVCache:
 
     def attend(self, layer: int, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, step: CacheStep, softmax_scale: Optional[float] = None,
                max_q_len: Optional[int] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
-        """the step's keys and values into the layer's cache, then its queries' attention (zeros for a request that was refused)"""
+        """the step's keys and values into the layer's cache, then its queries' attention (zeros for a request that was refused).  A step that brings a prompt while
+        other rows are idle should say so in max_q_len: the default takes every row to have a token (flash_attention_cached)"""
         self.append(layer, k, v, step)
         return flash_attention_cached(q, *self._layer[layer], self.block_tables, step.seq_lens, step.cu_new, softmax_scale, max_q_len, out, step.granted)

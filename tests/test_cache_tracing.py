@@ -104,3 +104,21 @@ def test_a_table_that_wants_a_gradient_is_refused():
     compiled = torch.compile(lambda t: rot.qk_norm_rope(x, x, None, None, t), backend="eager")
     with pytest.raises(Exception, match="no gradient for the table"):
         compiled(torch.zeros(8, 64, requires_grad=True))
+
+
+@pytest.mark.parametrize("tokens,told,used", [(5, None, 1), (8, None, 1), (12, None, 5), (500, None, 493), (500, 1, 1), (5, 5, 5)])
+def test_the_hint_that_a_call_goes_by(tokens, told, used):
+    """the documented guess, T - B + 1, and what the caller says in its place"""
+    class Hint(TorchDispatchMode):
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            if func._schema.name == "flash_attention_amd::cached":
+                seen.append(args[9])
+            return func(*args, **(kwargs or {}))
+
+    seen = []
+    with FakeTensorMode():
+        cache = kv.KVCache(1, 64, 2, 64, requests=8, max_tokens=600, block_size=16)
+        step = cache.step(torch.empty(8, device="cuda", dtype=torch.int32), tokens)
+        with Hint():
+            cache.attend(0, half(tokens, 4, 64), half(tokens, 2, 64), half(tokens, 2, 64), step, max_q_len=told)
+    assert seen == [used]

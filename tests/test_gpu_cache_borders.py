@@ -75,3 +75,12 @@ def test_refused_requests_between_served_ones(kv, dtype, D, hint, why):
         kv.flash_attention_cached(q.to(DEV), k_cache, v_cache, ks, vs, cache.block_tables, step.seq_lens, step.cu_new, granted=step.granted.long())
     with pytest.raises((ValueError, TypeError)):
         kv.flash_attention_cached(q.to(DEV), k_cache, v_cache, ks, vs, cache.block_tables, step.seq_lens, step.cu_new, granted=step.granted[1:])
+
+
+@BOTH
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_one_prompt_beside_idle_rows(kv, dtype, D):
+    """the default hint says one token each, and one request has them all"""
+    new = [0] * 40 + [37] + [0] * 9
+    check_attention(kv, [5] * 40 + [300] + [70] * 9, new, 2, 2, D, 16, dtype, seed=51)
+    check_attention(kv, [5] * 40 + [3000] + [70] * 9, new, 2, 2, D, 64, dtype, seed=52)
