@@ -245,6 +245,16 @@ def cache_append(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, k_cache:
     increment_version((k_cache, v_cache, k_scale, v_scale))
 
 
+def _rows_overlap(t):
+    """whether rows of [T, heads, D] with a unit stride on D can share memory: every larger stride has to step over all that the smaller ones span"""
+    span = t.shape[2]
+    for stride, n in sorted((s, n) for s, n in zip(t.stride()[:2], t.shape[:2]) if n > 1):
+        if stride < span:
+            return True
+        span += stride * (n - 1)
+    return False
+
+
 def _attn_call(q, k_cache, v_cache, k_scale, v_scale, block_tables, seq_lens, cu_q, softmax_scale, max_q_len, out, granted):
     name = "flash_attention_cached"
     key = (q.shape, q.stride(), q.dtype, None if out is None else (out.shape, out.stride(), out.dtype), max_q_len, k_cache.shape, k_cache.stride(), v_cache.shape, v_cache.stride(), k_cache.dtype,
@@ -260,6 +270,8 @@ def _attn_call(q, k_cache, v_cache, k_scale, v_scale, block_tables, seq_lens, cu
             raise ValueError(f"{name}: q must be [tokens, heads, head dim] (got {tuple(q.shape)})")
         if out is not None and (out.shape != q.shape or out.dtype != q.dtype or out.stride(2) != 1 or out.stride(0) % 8 or out.stride(1) % 8):
             raise ValueError(f"{name}: out must have q's shape and dtype and 16-byte rows")
+        if out is not None and _rows_overlap(out):
+            raise ValueError(f"{name}: rows of out must not share memory (strides {out.stride()})")
         T, H, D = q.shape
         heads_kv = k_cache.shape[1] if k_cache.ndim == 4 else 0
         if heads_kv < 1 or H % heads_kv:

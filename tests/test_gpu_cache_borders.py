@@ -84,3 +84,14 @@ def test_one_prompt_beside_idle_rows(kv, dtype, D):
     new = [0] * 40 + [37] + [0] * 9
     check_attention(kv, [5] * 40 + [300] + [70] * 9, new, 2, 2, D, 16, dtype, seed=51)
     check_attention(kv, [5] * 40 + [3000] + [70] * 9, new, 2, 2, D, 64, dtype, seed=52)
+
+
+def test_outputs_whose_rows_share_memory_are_refused(kv):
+    c = kv.KVCache(1, 8, 2, 64, requests=2, max_tokens=64, block_size=16)
+    q = torch.zeros(2, 4, 64, dtype=torch.float16, device=DEV)
+    args = (*c._layer[0], c.block_tables, ints([1, 1]), ints([0, 1, 2]))
+    room = torch.zeros(1024, dtype=torch.float16, device=DEV)
+    for strides in ((0, 64, 1), (256, 0, 1), (128, 64, 1)):
+        with pytest.raises(ValueError, match="share memory"):
+            kv.flash_attention_cached(q, *args, out=room.as_strided((2, 4, 64), strides))
+    kv.flash_attention_cached(q, *args, out=room.as_strided((2, 4, 64), (64, 128, 1)))
