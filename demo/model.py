@@ -13,8 +13,13 @@ import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
-from flash_attention_amd.kv_cache import KVCache
-from flash_attention_amd.rotary import qk_norm_rope, rotary_table
+try:
+    from flash_attention_amd.kv_cache import KVCache
+    from flash_attention_amd.rotary import qk_norm_rope, rotary_table
+except ModuleNotFoundError as e:        # (the plain model needs torch alone)
+    if e.name != "flash_attention_amd":
+        raise
+    KVCache = qk_norm_rope = rotary_table = None
 
 
 class CausalSelfAttention(nn.Module):
@@ -23,6 +28,8 @@ class CausalSelfAttention(nn.Module):
         n_kv_head = n_head if n_kv_head is None else n_kv_head
         if n_kv_head != n_head and not rotary:
             raise ValueError("n_kv_head needs rotary=True")
+        if rotary and qk_norm_rope is None:
+            raise ModuleNotFoundError("rotary=True needs flash_attention_amd on the path", name="flash_attention_amd")
         self.n_head, self.n_kv_head, self.n_embd, self.dropout, self.rotary = n_head, n_kv_head, n_embd, dropout, rotary
         self.c_attn = nn.Linear(n_embd, (n_head + 2 * n_kv_head) * (n_embd // n_head))
         self.c_proj = nn.Linear(n_embd, n_embd)
