@@ -90,7 +90,8 @@ class TinyGPT(nn.Module):
     def table(self, device):
         """cosines and sines of the block's positions: 32-bit whatever the model's type, and no parameter"""
         if self._table is None or self._table.device != device:
-            self._table = rotary_table(self.block, self.head_dim, device=device)
+            with torch.inference_mode(False):           # (one that an evaluation makes has to serve training too)
+                self._table = rotary_table(self.block, self.head_dim, device=device)
         return self._table
 
     def forward(self, idx):
