@@ -334,14 +334,13 @@ def stream_of(device: torch.device):
     return (_raw_stream(idx) if _raw_stream is not None else torch.cuda.current_stream(idx).cuda_stream), prev
 
 
-def through_dispatcher() -> bool:
-    """whether a call has to go through its registered op: it is compiled, traced, or a dispatch mode looks on (eager calls pass the dispatcher by)"""
-    return torch.compiler.is_compiling() or torch._C._len_torch_dispatch_stack() > 0
+# Eager calls pass the dispatcher by; one that is compiled (torch.compiler.is_compiling()) or that a dispatch mode looks on at, a tracer's among them, goes through its op.
+dispatch_modes = torch._C._len_torch_dispatch_stack
 
 
 def refuse_tangents(name, *tensors):
-    """no forward-mode derivative here: a dual tensor would lose its tangent without a word"""
-    if forward_ad._current_level >= 0 and any(t is not None and t.is_floating_point() and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+    """no forward-mode derivative here: a dual tensor would lose its tangent without a word (called inside of a forward-mode level only)"""
+    if any(t is not None and t.is_floating_point() and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
         raise ValueError(f"{name} has no forward-mode derivative")
 
 

@@ -7,6 +7,7 @@ import ctypes
 from typing import NamedTuple, Optional
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.graph import increment_version
 from torch.library import custom_op
 
@@ -128,7 +129,7 @@ def cache_tables(seq_lens: torch.Tensor, new_lens: torch.Tensor, block_tables: t
     A request is served whole or not at all (granted): its tokens have to end inside num_tokens, its blocks have to fit its table row, and the pool has
     to hold what all such requests up to and including it need.  Nothing is read back: look at `granted` when the host next waits for the device.
     """
-    dispatch = _native.through_dispatcher()
+    dispatch = torch.compiler.is_compiling() or _native.dispatch_modes()
     if dispatch:
         sizes = _check_tables(seq_lens, new_lens, block_tables, free_blocks, free_count, num_tokens, block_size, inplace)
     else:
@@ -238,8 +239,9 @@ def cache_append(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, k_cache:
     """
     if torch.is_grad_enabled() and (k.requires_grad or v.requires_grad or k_cache.requires_grad or v_cache.requires_grad or k_scale.requires_grad or v_scale.requires_grad):
         raise ValueError("cache_append has no gradient: call it under torch.no_grad()")
-    _native.refuse_tangents("cache_append", k, v, k_cache, v_cache, k_scale, v_scale)
-    if _native.through_dispatcher():
+    if forward_ad._current_level >= 0:
+        _native.refuse_tangents("cache_append", k, v, k_cache, v_cache, k_scale, v_scale)
+    if torch.compiler.is_compiling() or _native.dispatch_modes():
         return _append_op(k, v, slots, k_cache, v_cache, k_scale, v_scale)
     _append_call(k, v, slots, k_cache, v_cache, k_scale, v_scale)
     increment_version((k_cache, v_cache, k_scale, v_scale))
@@ -354,14 +356,15 @@ def flash_attention_cached(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torc
     if torch.is_grad_enabled() and (q.requires_grad or k_cache.requires_grad or v_cache.requires_grad or k_scale.requires_grad or v_scale.requires_grad
                                     or (out is not None and out.requires_grad)):
         raise ValueError("flash_attention_cached has no gradient: call it under torch.no_grad()")
-    _native.refuse_tangents("flash_attention_cached", q, k_cache, v_cache, k_scale, v_scale, out)
+    if forward_ad._current_level >= 0:
+        _native.refuse_tangents("flash_attention_cached", q, k_cache, v_cache, k_scale, v_scale, out)
     if softmax_scale is None:
         softmax_scale = q.shape[2] ** -0.5
     elif not 0.0 < softmax_scale < float("inf"):
         raise ValueError(f"flash_attention_cached: softmax_scale must be finite and > 0 (got {softmax_scale})")
     if max_q_len is None:
         max_q_len = max(1, q.shape[0] - seq_lens.shape[0] + 1) if seq_lens.ndim == 1 else 1
-    if _native.through_dispatcher():
+    if torch.compiler.is_compiling() or _native.dispatch_modes():
         if out is None:
             out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
         _attn_op(q, k_cache, v_cache, k_scale, v_scale, block_tables, seq_lens, cu_q, softmax_scale, max_q_len, out, granted)

@@ -8,6 +8,7 @@ import ctypes
 from typing import Optional, Tuple
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 from torch.library import custom_op
 
@@ -253,8 +254,9 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: Optional[torch.Tens
     grad = torch.is_grad_enabled()
     if grad and table.requires_grad:
         raise ValueError("qk_norm_rope has no gradient for the table")
-    _native.refuse_tangents("qk_norm_rope", q, k, q_weight, k_weight, table)
-    if _native.through_dispatcher():
+    if forward_ad._current_level >= 0:
+        _native.refuse_tangents("qk_norm_rope", q, k, q_weight, k_weight, table)
+    if torch.compiler.is_compiling() or _native.dispatch_modes():
         _check(q, k, q_weight, k_weight, table, positions)
         return _op(q, k, q_weight, k_weight, table, positions, float(eps), bool(interleaved))
     if grad and (q.requires_grad or k.requires_grad or (q_weight is not None and q_weight.requires_grad) or (k_weight is not None and k_weight.requires_grad)):
