@@ -330,7 +330,8 @@ int fa_cache_attn_granted(const void* q, void* out, const void* k_cache, const v
     fa::CacheAttnPlan plan;
     if (int rc = attn_plan(num_requests, num_tokens, heads, heads_kv, D, block_size, max_blocks, max_q_len, &plan)) return rc;
     if (int rc = cache_geometry(num_blocks, heads_kv, block_size, D, W, block_strides, k_cache, v_cache)) return rc;
-    if (!(softmax_scale > 0.f) || !isfinite(softmax_scale)) return fail(FA_ERR_BAD_SCALE, "softmax_scale must be finite and > 0 (got %g)", (double)softmax_scale);
+    const float scale_log2 = softmax_scale * 1.44269504088896340736f;
+    if (!(softmax_scale > 0.f) || !isfinite(scale_log2)) return fail(FA_ERR_BAD_SCALE, "softmax_scale must be > 0 and finite in powers of two (got %g)", (double)softmax_scale);
     if (table_stride < max_blocks || table_stride >= kMaxStride) return fail(FA_ERR_BAD_STRIDE, "table stride must hold a row");
     if (!aligned(q, 16) || !aligned(out, 16)) return fail(FA_ERR_MISALIGNED, "queries and output must be 16-byte aligned");
     for (int i = 0; i < 4; ++i) {
@@ -353,7 +354,7 @@ int fa_cache_attn_granted(const void* q, void* out, const void* k_cache, const v
     p.num_blocks = (int32_t)num_blocks; p.B = (int32_t)num_requests; p.T = (int32_t)num_tokens; p.Hq = (int32_t)heads; p.Hkv = (int32_t)heads_kv;
     p.group = (int32_t)(heads / heads_kv); p.D = (int32_t)D; p.width = (int32_t)max_blocks; p.shift = block_shift(block_size);
     p.grid = plan.grid; p.min_units = plan.min_units; p.whole = plan.whole; p.splits = plan.splits; p.max_tiles = plan.max_tiles; p.join_rows = plan.join_rows; p.join_chunks = plan.join_chunks;
-    p.scale_log2 = softmax_scale * 1.44269504088896340736f;
+    p.scale_log2 = scale_log2;
     return launched(fa::launch_cache_attn(p, plan, dtype, (hipStream_t)stream));
 }
 
