@@ -33,6 +33,7 @@ The cpu_baseline leg times the oracle's dense restatement of the reference CPU p
 """
 
 import argparse
+import gc
 import hashlib
 import json
 import os
@@ -817,6 +818,8 @@ def main():
                     pending[b] = None
 
     ramp_info = None
+    gc.collect()                 # (no collection of Python objects inside the timed region, and no idle time between the ramp and it)
+    gc.disable()
     step(0)                      # first call pays one-off host costs (library load, op registration)
     drain()
     sync()
@@ -859,6 +862,9 @@ def main():
                          "first_group_ms_per_step": round(durs[0][0], 4)}
     drain()
     sync()
+    ev0, ev1 = Ev(), Ev()
+    ev0.record()                 # (an event gets its handle with its first record: not inside the timed region)
+    ev1.record()
     for i in range(args.warmup):
         step(i)
     drain()
@@ -868,7 +874,6 @@ def main():
     sync()
 
     record[0] = dist_on and not strong          # per-launch events only where a collective shares the stream
-    ev0, ev1 = Ev(), Ev()
     t0 = time.perf_counter()
     ev0.record()
     for i in range(args.steps):
@@ -880,6 +885,7 @@ def main():
         dist.barrier()
     sync()
     elapsed = time.perf_counter() - t0
+    gc.enable()
     record[0] = False
     if kernel_events:      # N > 1, weak: kernel-only = events right around each launch (the waits on gathers sit before them)
         kernel_ms = sum(a.elapsed_time(b) for a, b in kernel_events) / len(kernel_events)
