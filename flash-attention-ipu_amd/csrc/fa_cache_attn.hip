@@ -26,7 +26,7 @@
 //                64 requests of 4600 tokens on average, 8 heads of 128: 105 us = 5.7 TB/s, every code read once, and 5 us for the join.
 //   tile kernel  128 rows per workgroup, 64 where no request has more (prompts): bound by the matrix pipe.  Four waves share a unit's operands,
 //                converted once into LDS in the very order in which the lanes read them.  Grids too small for the chip cut every tile's
-//                key range into `splits` parts.  Four prompts of 2048 over 8192 tokens, 32 / 8 heads: bf16 1014 TFLOP/s at width 128, 695 at 64, 638 at 256 (f16 1004, 682, 590)
+//                key range into `splits` parts.  Four prompts of 2048 over 8192 tokens, 32 / 8 heads: bf16 1020 TFLOP/s at width 128, 700 at 64, 600 at 192, 640 at 256 (f16 1000, 685, 560, 590)
 //                (matrix pipe 39 % busy, vector issue 41 %, LDS 51 %).
 // Stale codes behind a request's end are cleared before they meet a zero weight (0 * NaN), and a NaN code that only some rows of a unit may
 // see reaches those rows alone.

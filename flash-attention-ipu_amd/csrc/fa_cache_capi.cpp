@@ -155,7 +155,8 @@ int attn_plan(int64_t B, int64_t T, int64_t heads, int64_t heads_kv, int64_t D, 
         p.ws_prefix = p.ws_ml + slots * 16 * p.nr * 8;
     } else {
         // 128 rows per workgroup, or 64 where no request has more: 64 requests of 2048 tokens, width 128: 64 rows 72 us (with 128: 87), 80 rows 129 (88); width 256:
-        // 178 (267), 330 (269); four prompts of 2048 over 8192, width 256, f16: 536 TFLOP/s with 64, 576 with 128
+        // 178 (267), 330 (269); four prompts of 2048 over 8192, width 256, f16: 536 TFLOP/s with 64, 576 with 128 (590
+        // since its weights carry the value scale)
         p.nr = rows > 64 ? 2 : 1;
         const int64_t rows_wg = 64 * p.nr, bound = T * group / rows_wg + B;
         int64_t tiles = up(T * group, rows_wg);
