@@ -179,6 +179,9 @@ _op.register_autograd(_op_backward, setup_context=_op_setup)
 def _backward(ctx, dq_out, dk_out):
     q, k, q_weight, k_weight, table, positions = ctx.saved_tensors
     need = ctx.needs_input_grad
+    if torch.compiler.is_compiling() or _native.dispatch_modes():         # (a tracer that looks on at the backward alone)
+        dq, dk, dqw, dkw = _op_bwd(q, k, dq_out, dk_out, q_weight, k_weight, table, positions, ctx.eps, ctx.interleaved)
+        return dq, dk, dqw if need[2] else None, dkw if need[3] else None, None, None, None, None
     return (*_bwd_impl(q, k, dq_out, dk_out, q_weight, k_weight, table, positions, ctx.eps, ctx.interleaved, need[2], need[3]), None, None, None, None)
 
 

@@ -48,16 +48,17 @@ def test_a_traced_step_runs(kv, rot):
     assert torch.equal(got, want) and torch.equal(a.seq_lens, b.seq_lens) and torch.equal(a.block_tables, b.block_tables)
 
 
+class Log(TorchDispatchMode):
+    def __init__(self):
+        super().__init__()
+        self.names = []
+
+    def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+        self.names.append(func._schema.name)
+        return func(*args, **(kwargs or {}))
+
+
 def test_the_backward_is_dispatched(rot):
-    class Log(TorchDispatchMode):
-        def __init__(self):
-            super().__init__()
-            self.names = []
-
-        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
-            self.names.append(func._schema.name)
-            return func(*args, **(kwargs or {}))
-
     g = torch.Generator().manual_seed(1)
     leaves = [torch.randn(2, h, 10, 64, generator=g).half().to(DEV).requires_grad_() for h in (4, 2)] + [torch.ones(64, device=DEV).half().requires_grad_()]
     table = rot.rotary_table(20, 64, device=DEV)
@@ -68,6 +69,20 @@ def test_the_backward_is_dispatched(rot):
         got = run()
     assert [n for n in log.names if n.startswith("flash")] == ["flash_attention_amd::qk_norm_rope", "flash_attention_amd::qk_norm_rope_bwd"]
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_a_backward_alone_is_dispatched(rot):
+    """the mode is entered behind the forward"""
+    g = torch.Generator().manual_seed(2)
+    leaves = [torch.randn(2, h, 10, 64, generator=g).half().to(DEV).requires_grad_() for h in (4, 2)] + [torch.ones(64, device=DEV).half().requires_grad_()]
+    table = rot.rotary_table(20, 64, device=DEV)
+    for weights, wanted in (((leaves[2], None), leaves), ((None, leaves[2]), leaves), ((leaves[2], leaves[2].detach()), leaves), ((None, None), leaves[:2]), ((leaves[2].detach(), None), leaves[:1])):
+        out = rot.qk_norm_rope(*leaves[:2], *weights, table)
+        grads = [torch.randn(t.shape, generator=g).half().to(DEV) for t in out]
+        want = torch.autograd.grad(out, wanted, grads, retain_graph=True)
+        with Log() as log:
+            got = torch.autograd.grad(out, wanted, grads)
+        assert [n for n in log.names if n.startswith("flash")] == ["flash_attention_amd::qk_norm_rope_bwd"] and all(torch.equal(a, b) for a, b in zip(got, want))
 
 
 def test_changed_tensors_say_so(kv):
