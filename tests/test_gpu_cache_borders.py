@@ -95,3 +95,24 @@ def test_outputs_whose_rows_share_memory_are_refused(kv):
         with pytest.raises(ValueError, match="share memory"):
             kv.flash_attention_cached(q, *args, out=room.as_strided((2, 4, 64), strides))
     kv.flash_attention_cached(q, *args, out=room.as_strided((2, 4, 64), (64, 128, 1)))
+
+
+@BOTH
+@pytest.mark.parametrize("P", [16, 64, 128])
+@pytest.mark.parametrize("new", [1, 70])
+def test_blocks_of_a_larger_allocation(kv, dtype, P, new):
+    """a layer's blocks and scales as slices of tensors that hold more: strides between blocks of their own, codes and scales around them NaN"""
+    g = torch.Generator().manual_seed(61)
+    N, H, D = 24, 2, 128
+    plain = [torch.randint(0, 120, s, generator=g, dtype=torch.uint8).to(DEV) for s in ((N, H, P, D), (N, H, D, P))]
+    scales = [torch.exp2(torch.randint(-8, -4, (N, H), generator=g).float()).to(DEV) for _ in "kv"]
+    wide = [torch.full((N, 3, *t.shape[1:]), 0x7F, dtype=torch.uint8, device=DEV) for t in plain]
+    wide_scales = [torch.full((N, 3, H), float("nan"), device=DEV) for _ in "kv"]
+    for w, t in zip(wide + wide_scales, plain + scales):
+        w[:, 1] = t
+    tables, lens, cu = ints(np.random.default_rng(0).permutation(N).reshape(2, 12)), ints([12 * P - 3, 7 * P + 1]), ints([0, new, 2 * new])
+    q = torch.randn(2 * new, 4, D, generator=g).to(dtype).to(DEV)
+    fp8 = lambda ts: [t.view(torch.float8_e4m3fn) for t in ts]  # noqa: E731
+    want = kv.flash_attention_cached(q, *fp8(plain), *scales, tables, lens, cu, max_q_len=new)
+    got = kv.flash_attention_cached(q, *[t[:, 1] for t in fp8(wide)], *[t[:, 1] for t in wide_scales], tables, lens, cu, max_q_len=new)
+    assert torch.equal(got, want) and bool(torch.isfinite(want).all())

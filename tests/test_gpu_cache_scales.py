@@ -112,3 +112,23 @@ def test_light_weights_on_large_values(kv, dtype, P, n, below):
     k[-heavy * P:, 0] = -float(below)
     v[-heavy * P:] = codes((heavy * P, D), 20, 60, g).abs()
     check(kv, dtype, P, k, v, vs, n, n)
+
+
+@BOTH
+@BLOCKS
+@pytest.mark.parametrize("n", [1, 70])
+@pytest.mark.parametrize("scale", [0.0, 2.0 ** -100, 2.0 ** -70, 2.0 ** -64, 2.0 ** -40])
+@pytest.mark.parametrize("below", [0, 8])
+def test_weights_of_values_of_zero(kv, dtype, P, n, scale, below):
+    """blocks of zeros, whatever their scale, hold most of a row's weight: it stays in the sum"""
+    g = torch.Generator().manual_seed(below + 3)
+    blocks = max(6, 384 // P)
+    L = blocks * P - 5
+    k, v = codes((L, D), 0, 1, g), codes((L, D), 8, 100, g)
+    k[:, 0] = -float(below)
+    vs = torch.full((blocks,), 2.0 ** 6)
+    for b in (0, blocks // 2, blocks - 2):
+        vs[b] = scale
+        v[b * P:(b + 1) * P] = 0
+        k[b * P:(b + 1) * P, 0] = 0
+    check(kv, dtype, P, k, v, vs, n, n)
